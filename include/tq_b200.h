@@ -5,7 +5,7 @@
  * int32 status (0 = ok, negative = error, see TQ_ERR_*) and never throws.  The
  * caller owns all device buffers and passes the CUDA stream to launch on; kernels
  * are asynchronous on that stream.  The compute entry points (tq_pack, tq_decode_*,
- * tq_dequant, tq_key_norm_sum, tq_gather_wait) allocate nothing.  The calls that
+ * tq_dequant, tq_key_norm_sum, tq_gather_wait, tq_prompt_*, tq_tree_*, tq_cache_*) allocate nothing.  The calls that
  * allocate are: tq_ctx_create / tq_ctx_destroy (the device copy of the codec
  * tables), tq_peer_buffer_create / tq_peer_buffer_destroy (device memory that other
  * processes can map), and - only while tq_profile_enable is on - the decode calls,
@@ -55,6 +55,8 @@ extern "C" {
 
 #define TQ_HEAD_DIM 128
 #define TQ_MAX_GROUPS 8 /* query heads per KV head */
+#define TQ_MAX_PROMPT_GROUPS 64 /* query heads per KV head in prompt attention */
+#define TQ_MAX_TREE 64  /* drafted tokens per batch entry under a tree mask */
 
 typedef struct tq_ctx tq_ctx;
 typedef struct tq_gather_desc tq_gather_desc; /* KV-head sharding, defined below */
@@ -202,6 +204,62 @@ int32_t tq_dequant(tq_ctx *ctx, const tq_cache_desc *cache, int32_t which, int32
 int32_t tq_key_norm_sum(const tq_dense_desc *k, int32_t batch, int32_t heads, int32_t n_tokens,
                         double *sum_out, tq_stream stream);
 
+/* ---- Drafted tokens (no counterpart in the reference, whose decode step has one query token).
+ * A drafting loop packs n_nodes drafted tokens per batch entry with tq_pack, at tokens
+ * [tree_start, tree_start + n_nodes) of every row, attends all of them at once with tq_tree_attn, picks
+ * the ones it accepts and moves those behind their entry's history with tq_cache_keep_tokens.  Histories
+ * may differ in length from entry to entry; tree_start lies behind the longest of them.
+ *
+ * tq_tree_attn: q [batch, q_heads, n_nodes, 128] and out of the same shape (fp16 or bf16, the same dtype; outer
+ * strides in elements, multiples of 8, data 16-byte aligned; stride_h / stride_t of out must keep its vectors
+ * apart).  Node i of entry b attends the tokens [seq_start[b], lengths[b]) of the cache's rows and the drafted
+ * tokens j whose bit j is set in tree_mask[b * n_nodes + i] (itself included only if bit i is set; at most
+ * TQ_MAX_TREE nodes).  tree_mask NULL: a chain, node i sees the drafted tokens 0 .. i, any n_nodes.  lengths:
+ * device int32 [batch], clamped to [0, tree_start]; NULL: tree_start for all.  seq_start clamped to
+ * [0, length].  A node that sees nothing gets zeros.  Softmax scale 1/sqrt(128). */
+size_t tq_tree_workspace_bytes(tq_ctx *ctx, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_nodes,
+                               int32_t tree_start);
+int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_heads, int32_t n_nodes, const tq_cache_desc *cache,
+                     int32_t tree_start, const int32_t *lengths, const uint64_t *tree_mask, void *workspace,
+                     size_t workspace_bytes, const tq_dense_desc *out, tq_stream stream);
+/* Token tree_start + path[b * path_len + i] of every row of entry b moves to token lengths[b] + i, for i < counts[b],
+ * in all streams; lengths_out[b] = lengths[b] + counts[b].  All four are device int32 arrays; lengths_out is another one
+ * than lengths.  Paths ascend strictly.  An entry whose path, count or length is out of range stays as it is
+ * (tq_device_status 7). */
+int32_t tq_cache_keep_tokens(tq_ctx *ctx, const tq_cache_desc *cache, int32_t tree_start, const int32_t *path,
+                             int32_t path_len, const int32_t *counts, const int32_t *lengths, int32_t *lengths_out,
+                             tq_stream stream);
+/* Row b of dst becomes what row index[b] of src holds, tokens [lo, hi) of all streams and KV heads, for every b of
+ * dst->batch (index: device int64).  src and dst are two caches of the context's codec with the same number of KV
+ * heads, or the same one: every row is then read before any changes, so index may permute rows and name one several times;
+ * at most 448 rows in place.  seq_start_out (optional, device int32 [dst->batch], not src->seq_start itself): the row
+ * offsets that go with it.  A row whose index is out of range is left alone (tq_device_status 7). */
+int32_t tq_cache_select_rows(tq_ctx *ctx, const tq_cache_desc *src, const tq_cache_desc *dst, const int64_t *index,
+                             int32_t lo, int32_t hi, int32_t *seq_start_out, tq_stream stream);
+
+/* ---- Attention of a whole prompt over dense keys and values (the reference runs the model's own attention here,
+ * src/turboquant/runtime/generation.py:91).  No context: nothing of it depends on a codec; the launch goes to the current
+ * device.  q / out [batch, q_heads, n_q, 128], k / v [batch, kv_heads, n_kv, 128], all fp16 or all bf16; outer strides
+ * in elements, multiples of 8 (anything where the size is 1), data 16-byte aligned.  Query i sees the keys
+ * [seq_start[b], i + n_kv - n_q] (causal; needs n_kv >= n_q) or [seq_start[b], n_kv).  seq_start: optional device int32
+ * [batch], clamped to [0, n_kv].  A query that sees nothing gets zeros.  Keys and values before seq_start are not looked at: they may hold
+ * anything.  Logits are scale * (q . k).
+ *
+ * tq_prompt_attn_packed: n_seqs sequences end to end, q / out [total, q_heads, 128], k / v [total, kv_heads, 128]
+ * (stride_b unused); sequence s is the tokens [cu_seqlens[s], cu_seqlens[s + 1]) (device int32 [n_seqs + 1], ascending,
+ * not above total), of at most max_seqlen tokens; tokens beyond that, and those behind the last sequence, are left as
+ * they were in out.
+ * tq_prompt_status: synchronises with the current device; 0, or 1 when a kernel's bounded wait ran out (sticky). */
+size_t tq_prompt_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv);
+int32_t tq_prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int32_t batch,
+                       int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv, const int32_t *seq_start, float scale,
+                       int32_t causal, void *workspace, size_t workspace_bytes, const tq_dense_desc *out, tq_stream stream);
+int32_t tq_prompt_attn_packed(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int32_t n_seqs,
+                              int32_t total, int32_t q_heads, int32_t kv_heads, const int32_t *cu_seqlens,
+                              int32_t max_seqlen, float scale, int32_t causal, void *workspace, size_t workspace_bytes,
+                              const tq_dense_desc *out, tq_stream stream);
+int32_t tq_prompt_status(int32_t *status_out);
+
 /* ---- KV-head sharding over the GPUs of one box (no counterpart in the reference, which is
  * single-GPU).  Rank r serves kv_heads / world KV heads and their query heads; the only exchange
  * per decode step is the per-head attention outputs.  tq_decode_attn_gather fuses that exchange
@@ -311,7 +369,8 @@ int32_t tq_set_wait_limit_ms(tq_ctx *ctx, int32_t limit_ms);
  * 1 = a decode kernel's wait ran out; 2 = a decode kernel found that its shared-memory layout
  * does not fit and did not run; 3 = the encoder's wait ran out; 4 = an append addressed a
  * token past the cache's capacity and was dropped; 5 = tq_gather_wait gave up waiting for a peer;
- * 6 = (bounds-checked build only) a kernel was about to read or write outside a buffer and did not.
+ * 6 = (bounds-checked build only) a kernel was about to read or write outside a buffer and did not;
+ * 7 = a move of cached rows or tokens named one that does not exist and was dropped; 8 = the wait of tq_tree_attn's kernel ran out.
  * The word is sticky for the context. */
 int32_t tq_device_status(tq_ctx *ctx, int32_t *status_out);
 

@@ -42,6 +42,26 @@ def dense_desc(t: torch.Tensor) -> ffi.DenseDesc:
     return ffi.DenseDesc(t.data_ptr(), tq_dtype(t.dtype), t.stride(0), t.stride(1), t.stride(2))
 
 
+def aligned_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when kernels that move 16 bytes at a time can address it (contiguous last axis, rows on 16-byte
+    boundaries, no axis repeated by a stride of 0), else a contiguous copy."""
+    step = 16 // t.element_size()
+    fits = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        n <= 1 or (s > 0 and s % step == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
+
+
+def strided_desc(t: torch.Tensor) -> ffi.DenseDesc:
+    """``dense_desc`` of an ``aligned_view``: an axis of one element has no stride of its own."""
+    strides = [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    return ffi.DenseDesc(t.data_ptr(), tq_dtype(t.dtype), *strides)
+
+
+def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ffi.TQError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
 class Codec:
     """Owns one ``tq_ctx`` on one CUDA device."""
 
@@ -131,6 +151,8 @@ class Codec:
         4: "an append addressed a token past the cache's capacity and was dropped",
         5: "the wait for a peer's attention outputs ran out (tq_gather_wait)",
         6: "the bounds-checked build stopped a kernel from reading or writing outside a buffer",
+        7: "a move of cached rows or tokens named one that does not exist and was dropped",
+        8: "the wait of a drafted-token attention kernel ran out",
     }
 
     def raise_on_device_status(self, where: str) -> None:

@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("TQ_B200_LIBRARY") or os.path.join(_PKG, "libtq_b200.s
 
 TQ_DTYPE_F32, TQ_DTYPE_F16, TQ_DTYPE_BF16 = 0, 1, 2
 TQ_MAX_GROUPS = 8
+TQ_MAX_TREE = 64
 
 EXPORTS = (
     "tq_abi_version", "tq_last_cuda_error", "tq_ctx_create", "tq_ctx_destroy", "tq_pack",
@@ -25,6 +26,8 @@ EXPORTS = (
     "tq_peer_buffer_create", "tq_peer_buffer_open", "tq_peer_buffer_close", "tq_peer_buffer_destroy",
     "tq_decode_attn_gather", "tq_gather_wait", "tq_decode_step_host_gather", "tq_set_wait_limit_ms", "tq_decode_attn_f32out",
     "tq_parts_exchange_bytes", "tq_decode_attn_parts", "tq_decode_parts_finish",
+    "tq_tree_workspace_bytes", "tq_tree_attn", "tq_cache_keep_tokens", "tq_cache_select_rows",
+    "tq_prompt_workspace_bytes", "tq_prompt_attn", "tq_prompt_attn_packed", "tq_prompt_status",
 )
 
 _ERRORS = {-1: "bad argument", -2: "unsupported shape or mode", -3: "CUDA error", -4: "workspace too small"}
@@ -150,6 +153,24 @@ def lib() -> C.CDLL:
     L.tq_decode_parts_finish.argtypes = [C.c_void_p, C.POINTER(GatherDesc), C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                          C.c_void_p, C.c_void_p]
     L.tq_decode_parts_finish.restype = C.c_int32
+    dense, cache = C.POINTER(DenseDesc), C.POINTER(CacheDesc)
+    L.tq_tree_workspace_bytes.argtypes = [C.c_void_p] + [C.c_int32] * 5
+    L.tq_tree_workspace_bytes.restype = C.c_size_t
+    L.tq_tree_attn.argtypes = [C.c_void_p, dense, C.c_int32, C.c_int32, cache, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                               C.c_size_t, dense, C.c_void_p]
+    L.tq_cache_keep_tokens.argtypes = [C.c_void_p, cache, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p]
+    L.tq_cache_select_rows.argtypes = [C.c_void_p, cache, cache, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]
+    L.tq_prompt_workspace_bytes.argtypes = [C.c_int32] * 5
+    L.tq_prompt_workspace_bytes.restype = C.c_size_t
+    L.tq_prompt_attn.argtypes = [dense, dense, dense] + [C.c_int32] * 5 + [C.c_void_p, C.c_float, C.c_int32, C.c_void_p,
+                                                                          C.c_size_t, dense, C.c_void_p]
+    L.tq_prompt_attn_packed.argtypes = [dense, dense, dense] + [C.c_int32] * 4 + [C.c_void_p, C.c_int32, C.c_float, C.c_int32,
+                                                                                 C.c_void_p, C.c_size_t, dense, C.c_void_p]
+    L.tq_prompt_status.argtypes = [C.POINTER(C.c_int32)]
+    for name in ("tq_tree_attn", "tq_cache_keep_tokens", "tq_cache_select_rows", "tq_prompt_attn", "tq_prompt_attn_packed",
+                 "tq_prompt_status"):
+        getattr(L, name).restype = C.c_int32
     L.tq_set_wait_limit_ms.argtypes = [C.c_void_p, C.c_int32]
     L.tq_set_wait_limit_ms.restype = C.c_int32
     for name in ("tq_peer_buffer_create", "tq_peer_buffer_open", "tq_peer_buffer_close", "tq_peer_buffer_destroy",

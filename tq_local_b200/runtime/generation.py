@@ -18,6 +18,7 @@ on the host side of the hot path:
 from __future__ import annotations
 
 import time
+from contextlib import contextmanager
 from dataclasses import asdict, dataclass
 from typing import Any
 
@@ -96,6 +97,29 @@ def _prefill(model, inputs, cache=None):
         if cache is not None and any(layer.is_initialized for layer in cache.layers):
             raise  # the cache already holds part of the prompt: a second pass would store it twice
         return model(**inputs, use_cache=True, **extra)
+
+
+@contextmanager
+def _prompt_kernels(model, inputs, enabled: bool):
+    """The prompt pass inside runs on this library's prompt attention where it computes what the model asks for (see
+    ``prompt_attention.turboquant_prompt_forward``).  Only causal, at most left-padded batches qualify."""
+    from tq_local_b200.runtime.packed_qmse_cache import is_left_padding_mask
+
+    config, mask = getattr(model, "config", None), inputs.get("attention_mask")
+    if not enabled or config is None or (mask is not None and not is_left_padding_mask(mask)):
+        yield
+        return
+    from tq_local_b200.runtime.prompt_attention import raise_on_status, register_prompt_backend
+
+    register_prompt_backend()
+    previous = getattr(config, "_attn_implementation", None)
+    config._attn_implementation = "turboquant_prompt"
+    try:
+        yield
+    finally:
+        config._attn_implementation = previous or "sdpa"
+    if inputs["input_ids"].device.type == "cuda":
+        raise_on_status(inputs["input_ids"].device, "prompt pass")
 
 
 def raise_on_device_status(layers, where: str) -> None:
@@ -304,6 +328,7 @@ def greedy_decode_with_prefill_cache(
     shard=None,
     use_cuda_graph: bool | None = None,
     prefill_block_tokens: int | None = None,
+    prompt_attention: bool = False,
 ) -> GenerationOutput:
     import torch
 
@@ -337,14 +362,17 @@ def greedy_decode_with_prefill_cache(
             rows_per_block = max(1, block_tokens // max(int(ids.shape[1]), 1))
             if rows_per_block < int(ids.shape[0]):
                 threshold = _auto_norm_threshold(qmse_bits, head_dim) if norm_guard else float("inf")
-                last_logits = _prefill_in_row_blocks(model, inputs, packed_cache, threshold, rows_per_block)
+                with _prompt_kernels(model, inputs, prompt_attention):
+                    last_logits = _prefill_in_row_blocks(model, inputs, packed_cache, threshold, rows_per_block)
                 cache = packed_cache
             else:
-                outputs = _prefill(model, inputs, packed_cache)
+                with _prompt_kernels(model, inputs, prompt_attention):
+                    outputs = _prefill(model, inputs, packed_cache)
                 cache, last_logits = outputs.past_key_values, outputs.logits[:, -1, :]
                 del outputs
         else:
-            outputs = _prefill(model, inputs)
+            with _prompt_kernels(model, inputs, prompt_attention):
+                outputs = _prefill(model, inputs)
             cache, last_logits = outputs.past_key_values, outputs.logits[:, -1, :]
             del outputs
         next_token = torch.argmax(last_logits, dim=-1, keepdim=True)

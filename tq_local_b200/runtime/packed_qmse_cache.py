@@ -128,6 +128,10 @@ class _GrowingDense:
     def view(self) -> torch.Tensor | None:
         return None if self.buf is None else self.buf[:, :, :self.length]
 
+    def take_rows(self, index: torch.Tensor) -> None:
+        if self.buf is not None:
+            self.buf = self.buf.index_select(0, index.to(self.buf.device))
+
 
 class PackedMSELayer(CacheLayerMixin):
     """One layer of the packed cache (reference: packed_qmse_cache.py:163-885)."""
@@ -180,6 +184,7 @@ class PackedMSELayer(CacheLayerMixin):
         self._static_kv: tuple[torch.Tensor, torch.Tensor] | None = None
         self._static_gather = None
         self._split = False  # outlier-channel split in use (see lazy_initialization)
+        self._tree: tuple[torch.Tensor | None, torch.Tensor | None] | None = None  # see bind_tree
 
     # ---------------------------------------------------------------- reference attributes
     @property
@@ -543,6 +548,8 @@ class PackedMSELayer(CacheLayerMixin):
             return self.store.decode_step_dev(self.shard.local_q(query_states, self._kv_heads_total),
                                               self.shard.local_kv(k_new), self.shard.local_kv(v_new), self._static_pos,
                                               gather=self._static_gather)
+        if self._tree is not None:
+            return self.attend_tree(query_states, *self._tree)
         b, hq, sq, d = query_states.shape
         q_local = self.shard.local_q(query_states, self._kv_heads_total)
         if self.seq_parts > 1:
@@ -568,6 +575,85 @@ class PackedMSELayer(CacheLayerMixin):
             outs.append(out)
         out = outs[0] if sq == 1 else torch.cat(outs, dim=2)
         return self.shard.gather_heads(out)
+
+    # ---------------------------------------------------------------- drafted tokens
+    def _plain_store(self, what: str) -> PackedStore:
+        """The store of a layer all of whose tokens are packed ones of this rank."""
+        if self.store is None or self._force_dense:
+            raise RuntimeError(f"{what} needs a packed (non-dense) layer")
+        if self._split or self.seq_parts > 1 or self._dense_k.length:
+            raise NotImplementedError(f"{what} is available for layers whose tokens are all packed, without an outlier split and not "
+                                      "shared out over several ranks")
+        return self.store
+
+    def bind_tree(self, tree_mask: torch.Tensor | None, lengths: torch.Tensor | None = None) -> None:
+        """The next model steps are of drafted tokens: a step's T tokens are appended as usual and ``attend`` lets each
+        see its history and what ``tree_mask`` says of the others (see ``PackedStore.tree_attn``) instead of going
+        through them one at a time.  ``unbind_tree`` ends this."""
+        self._plain_store("bind_tree")
+        if not self.quantize_decode or self._static_pos is not None:
+            raise RuntimeError("drafted tokens are packed ones: quantize_decode=True, outside a static decode")
+        self._tree = (tree_mask, lengths)
+
+    def unbind_tree(self) -> None:
+        self._tree = None
+
+    def attend_tree(self, query_states: torch.Tensor, tree_mask: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                    tree_start: int | None = None) -> torch.Tensor:
+        """Attention of the drafted tokens at ``[tree_start, tree_start + T)`` (default: the last T packed), ``query_states``
+        [B, Hq, T, D] in and out."""
+        store = self._plain_store("attend_tree")
+        out = store.tree_attn(self.shard.local_q(query_states, self._kv_heads_total), tree_mask, tree_start=tree_start, lengths=lengths)
+        return self.shard.gather_heads(out)
+
+    def keep_tokens(self, path: torch.Tensor, counts: torch.Tensor, *, tree_start: int, lengths: torch.Tensor) -> torch.Tensor:
+        """``PackedStore.keep_tokens`` of this layer; ``crop`` then gives up what lies behind the longest row."""
+        return self._plain_store("keep_tokens").keep_tokens(path, counts, tree_start=tree_start, lengths=lengths)
+
+    # ---------------------------------------------------------------- rows and lengths (the hooks of transformers' Cache)
+    def _before_rows_move(self, what: str) -> None:
+        if self._split:
+            raise NotImplementedError(f"{what} is not available with an outlier-channel split")
+        if self._static_pos is not None:
+            raise RuntimeError(f"{what} inside a static decode")
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Row ``b`` of the cache becomes what row ``beam_idx[b]`` was."""
+        self._before_rows_move("reorder_cache")
+        if self.store is not None:
+            self.store.select_rows(beam_idx.to(self.device))
+        self._dense_k.take_rows(beam_idx), self._dense_v.take_rows(beam_idx)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        """The cache of a batch of ``len(indices)`` rows: row ``i`` is what row ``indices[i]`` was."""
+        self._before_rows_move("batch_select_indices")
+        if self.store is not None:
+            self.store = self.store.take_rows(indices.to(self.device))
+        self._dense_k.take_rows(indices), self._dense_v.take_rows(indices)
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        """Every row ``repeats`` times, side by side."""
+        batch = self.store.batch if self.store is not None else 0 if self._dense_k.buf is None else int(self._dense_k.buf.shape[0])
+        if batch:
+            self.batch_select_indices(torch.arange(batch, device=self.device).repeat_interleave(int(repeats)))
+
+    def crop(self, max_length: int) -> None:
+        """Keep the first ``max_length`` tokens (negative: give up the last ``-max_length``)."""
+        if self.seq_parts > 1:
+            raise NotImplementedError("crop is not available when several ranks share a KV head")
+        if self._static_pos is not None:
+            raise RuntimeError("crop inside a static decode")
+        seen = self.get_seq_length()
+        keep = max(seen + max_length, 0) if max_length < 0 else int(max_length)
+        if keep >= seen:
+            return
+        packed = self.packed_seq_length()
+        if self.store is not None and keep < packed:
+            if self._split:
+                raise NotImplementedError("crop is not available with an outlier-channel split")
+            self.store.truncate(keep)
+        self._dense_k.length = self._dense_v.length = max(keep - packed, 0)
+        self._tokens_seen = keep
 
     def attend_with_new_tokens(self, query_states: torch.Tensor, new_key: torch.Tensor, new_value: torch.Tensor,
                                attention_mask: torch.Tensor | None = None) -> torch.Tensor:

@@ -23,7 +23,7 @@ import ctypes as C
 import torch
 
 from tq_local_b200.runtime import ffi
-from tq_local_b200.runtime.codec import Codec, dense_desc, tq_dtype
+from tq_local_b200.runtime.codec import Codec, aligned_view, dense_desc, refuse_grad, strided_desc, tq_dtype
 
 
 def _round_up(n: int, m: int) -> int:
@@ -410,6 +410,111 @@ class PackedStore:
                                                    None if gdesc is None else C.byref(gdesc), self._stream_ptr()),
                       "tq_decode_step_dev")
         return out
+
+    # ------------------------------------------------------------------ drafted tokens
+    def _int32(self, t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
+        if t.dtype != torch.int32 or t.device != self.codec.device or tuple(t.shape) != shape:
+            raise ValueError(f"{what} must be an int32 tensor {list(shape)} on {self.codec.device}")
+        return t.contiguous()
+
+    def tree_attn(self, q: torch.Tensor, tree_mask: torch.Tensor | None = None, *, tree_start: int | None = None,
+                  lengths: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of the T drafted tokens that every row holds at tokens ``[tree_start, tree_start + T)`` (default: the
+        last T packed): ``q`` [B, Hq, T, 128] (fp16 or bf16) -> [B, Hq, T, 128], a view of [B, T, Hq, 128].  Entry ``b`` attends its
+        history ``[seq_start[b], lengths[b])`` (``lengths``: int32 [B] on the device; default: all of ``[0, tree_start)``) and,
+        of the drafted tokens, those whose bits are set in ``tree_mask`` (int64 [B, T], or [T] for all rows; bit j of
+        word i: node i sees node j; T at most 64).  Without a mask they are a chain: node i sees nodes 0 .. i, any T.  With
+        T = 1 and no mask this is single-token decoding of rows of different lengths."""
+        if q.dim() != 4 or q.shape[0] != self.batch or q.shape[-1] != 128 or q.shape[1] % self.kv_heads:
+            raise ValueError(f"expected queries [B={self.batch}, Hq, T, 128] with Hq a multiple of {self.kv_heads}, got {tuple(q.shape)}")
+        if q.device != self.codec.device:
+            raise ffi.TQError(f"tensor on {q.device}, cache on {self.codec.device}")
+        refuse_grad("tree_attn", q)
+        b, hq, t = int(q.shape[0]), int(q.shape[1]), int(q.shape[2])
+        start = self.length - t if tree_start is None else int(tree_start)
+        if start < 0 or start + t > self.length:
+            raise ValueError(f"drafted tokens [{start}, {start + t}) are not among the {self.length} packed ones")
+        if lengths is not None:
+            lengths = self._int32(lengths, (b,), "lengths")
+        if tree_mask is not None:
+            if tree_mask.dtype != torch.int64 or tree_mask.device != self.codec.device or tuple(tree_mask.shape) not in ((b, t), (t,)):
+                raise ValueError(f"tree_mask must be an int64 tensor [{b}, {t}] or [{t}] on {self.codec.device}")
+            tree_mask = (tree_mask if tree_mask.dim() == 2 else tree_mask.expand(b, t)).contiguous()
+        if out is None:
+            out = torch.empty(b, t, hq, 128, dtype=q.dtype, device=q.device).transpose(1, 2)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or aligned_view(out) is not out:
+            raise ValueError("out must have the queries' shape, dtype and device, with rows on 16-byte boundaries")
+        if t == 0:
+            return out
+        q = aligned_view(q)
+        need = int(ffi.lib().tq_tree_workspace_bytes(self.codec.handle, b, hq, self.kv_heads, t, start))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        qd, od = strided_desc(q), strided_desc(out)
+        self._call("tq_tree_attn", self.codec.handle, C.byref(qd), hq, t, self._desc_ref, start,
+                   None if lengths is None else lengths.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(),
+                   None if ws is None else ws.data_ptr(), need, C.byref(od))
+        return out
+
+    def keep_tokens(self, path: torch.Tensor, counts: torch.Tensor, *, tree_start: int, lengths: torch.Tensor) -> torch.Tensor:
+        """Move the accepted drafted tokens behind their histories: token ``tree_start + path[b, i]`` of row ``b`` goes to token
+        ``lengths[b] + i`` for ``i < counts[b]`` (``path`` int32 [B, P], ascending in every row; ``counts``, ``lengths`` int32
+        [B]).  Returns the new lengths, int32 [B]; ``length`` is the host's to set (``truncate``) once it knows the longest.
+        A row whose path or length is out of range stays as it is and is reported (device status 7)."""
+        b = self.batch
+        if path.dim() != 2:
+            raise ValueError(f"path must be an int32 tensor [{b}, P]")
+        path = self._int32(path, (b, int(path.shape[1])), "path")
+        counts, lengths = self._int32(counts, (b,), "counts"), self._int32(lengths, (b,), "lengths")
+        if not 0 <= int(tree_start) <= self.length:
+            raise ValueError(f"tree_start {tree_start} is not among the {self.length} packed tokens")
+        if path.shape[1] == 0:
+            return lengths.clone()
+        out = torch.empty_like(lengths)
+        self._call("tq_cache_keep_tokens", self.codec.handle, self._desc_ref, int(tree_start), path.data_ptr(), int(path.shape[1]),
+                   counts.data_ptr(), lengths.data_ptr(), out.data_ptr())
+        return out
+
+    def truncate(self, length: int) -> None:
+        """Give up the tokens from ``length`` on; their room is used by what is packed next."""
+        if not 0 <= int(length) <= self.length:
+            raise ValueError(f"cannot truncate {self.length} tokens to {length}")
+        self.length = int(length)
+
+    # ------------------------------------------------------------------ rows
+    def _index(self, index: torch.Tensor) -> torch.Tensor:
+        if index.dim() != 1 or index.dtype not in (torch.int32, torch.int64) or index.device != self.codec.device:
+            raise ValueError(f"index must be a 1-D int32 or int64 tensor on {self.codec.device}")
+        return index.to(torch.int64).contiguous()
+
+    def select_rows(self, index: torch.Tensor, lo: int = 0, hi: int | None = None) -> None:
+        """Row ``b`` becomes what row ``index[b]`` was (int32 or int64 [B] on the device): a beam search's reordering.  Only tokens
+        ``[lo, hi)`` are moved (default: all packed ones), for rows that share what lies before ``lo``; per-row offsets
+        (``set_seq_start``) go along.  A row whose index is out of range stays as it is and is reported (device status 7)."""
+        index = self._index(index)
+        hi = self.length if hi is None else int(hi)
+        if index.numel() != self.batch or not 0 <= int(lo) <= hi <= self.length:
+            raise ValueError(f"select_rows takes {self.batch} rows and tokens within [0, {self.length}), got {index.numel()} and [{lo}, {hi})")
+        starts = None if self._seq_start is None else torch.empty_like(self._seq_start)
+        self._call("tq_cache_select_rows", self.codec.handle, self._desc_ref, self._desc_ref, index.data_ptr(), int(lo), hi,
+                   None if starts is None else starts.data_ptr())
+        if starts is not None:
+            self.set_seq_start(starts)
+
+    def take_rows(self, index: torch.Tensor, capacity: int | None = None) -> "PackedStore":
+        """A new store whose row ``i`` holds what row ``index[i]`` of this one holds: a batch that forks, grows or shrinks.  Rows
+        whose index is out of range hold nothing that is defined and are reported (device status 7)."""
+        index = self._index(index)
+        if index.numel() == 0:
+            raise ValueError("take_rows needs at least one row")
+        other = PackedStore(self.codec, int(index.numel()), self.kv_heads, max(self.length, self.capacity if capacity is None else int(capacity)))
+        starts = None
+        if self._seq_start is not None:
+            starts = torch.empty(other.batch, dtype=torch.int32, device=self.codec.device)
+        self._call("tq_cache_select_rows", self.codec.handle, self._desc_ref, other._desc_ref, index.data_ptr(), 0, self.length,
+                   None if starts is None else starts.data_ptr())
+        other.length = self.length
+        other.set_seq_start(starts)
+        return other
 
     def dequant(self, which: str, lo: int = 0, hi: int | None = None,
                 dtype: torch.dtype = torch.float32) -> torch.Tensor:

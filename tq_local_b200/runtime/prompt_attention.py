@@ -1,0 +1,159 @@
+"""Attention of a whole prompt over its dense keys and values (``tq_prompt_attn``).
+
+The prompt pass of a packed-cache generation attends dense tensors; these are its kernels: causal, with grouped heads, over a
+left-padded batch, a chunk of a prompt behind keys that are there already, or sequences of different lengths laid end to end.
+``"turboquant_prompt"`` is the HF attention backend that calls them (``activate(..., prompt_attention=True)``).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from tq_local_b200.runtime import ffi
+from tq_local_b200.runtime.codec import aligned_view, refuse_grad, strided_desc
+
+
+def _check(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, dims: int, heads_axis: int) -> None:
+    shapes = f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}"
+    if query.dim() != dims or key.dim() != dims or key.shape != value.shape or query.shape[-1] != 128 or key.shape[-1] != 128:
+        raise ValueError(f"expected queries, keys and values of {dims} axes with 128 coordinates, keys and values alike; got {shapes}")
+    hq, hkv = int(query.shape[heads_axis]), int(key.shape[heads_axis])
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError(f"query heads must be a multiple of KV heads, got {shapes}")
+    if query.device.type != "cuda":
+        raise ffi.TQError("TurboQuant-B200 runs on CUDA devices only; there is no CPU path")
+    if key.device != query.device or value.device != query.device:
+        raise ffi.TQError(f"queries on {query.device}, keys on {key.device}, values on {value.device}")
+    if query.dtype not in (torch.float16, torch.bfloat16) or key.dtype != query.dtype or value.dtype != query.dtype:
+        raise TypeError(f"expected float16 or bfloat16 for all three, got {query.dtype}, {key.dtype}, {value.dtype}")
+    refuse_grad("prompt attention", query, key, value)
+
+
+def _int32(t: torch.Tensor, shape: tuple, device: torch.device, what: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+        raise ValueError(f"{what} must be an int32 tensor {list(shape)} on {device}")
+    return t.contiguous()
+
+
+def _output(out: torch.Tensor | None, query: torch.Tensor, make) -> torch.Tensor:
+    if out is None:
+        return make()
+    if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or aligned_view(out) is not out:
+        raise ValueError("out must have the queries' shape, dtype and device, with rows on 16-byte boundaries")
+    return out
+
+
+def _launch(name: str, device: torch.device, workspace_args: tuple, *args_of_workspace_and_stream) -> None:
+    before, after = args_of_workspace_and_stream
+    lib = ffi.lib()
+    need = int(lib.tq_prompt_workspace_bytes(*workspace_args))
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    args = (*before, None if ws is None else ws.data_ptr(), need, *after, torch.cuda.current_stream(device).cuda_stream)
+    if torch.cuda.current_device() == device.index:
+        status = getattr(lib, name)(*args)
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib, name)(*args)
+    ffi.check(status, name)
+
+
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
+                     causal: bool = True, seq_start: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``query`` [B, Hq, Sq, 128], ``key`` / ``value`` [B, Hkv, Skv, 128] (fp16 or bf16, any outer strides) -> [B, Hq, Sq, 128], a view of
+    [B, Sq, Hq, 128].  Causal: query ``i`` sees the keys up to ``i + Skv - Sq`` (so ``Sq`` < ``Skv`` is a chunk behind
+    ``Skv - Sq`` earlier tokens).  ``seq_start`` (int32 [B] on the device): entry ``b`` attends keys from there on, a
+    left-padded batch; a query that sees no key gets zeros.  ``scale`` defaults to 1/sqrt(128)."""
+    _check(query, key, value, 4, 1)
+    b, hq, n_q = int(query.shape[0]), int(query.shape[1]), int(query.shape[2])
+    hkv, n_kv = int(key.shape[1]), int(key.shape[2])
+    if key.shape[0] != b or (causal and n_kv < n_q):
+        raise ValueError(f"keys {tuple(key.shape)} do not go with queries {tuple(query.shape)}" + (" under a causal mask" if causal else ""))
+    if seq_start is not None:
+        seq_start = _int32(seq_start, (b,), query.device, "seq_start")
+    out = _output(out, query, lambda: torch.empty(b, n_q, hq, 128, dtype=query.dtype, device=query.device).transpose(1, 2))
+    if out.numel() == 0:
+        return out
+    if n_kv == 0:
+        return out.zero_()
+    q, k, v = aligned_view(query), aligned_view(key), aligned_view(value)
+    qd, kd, vd, od = strided_desc(q), strided_desc(k), strided_desc(v), strided_desc(out)
+    _launch("tq_prompt_attn", query.device, (b, hq, hkv, n_q, n_kv),
+            (C.byref(qd), C.byref(kd), C.byref(vd), b, hq, hkv, n_q, n_kv, None if seq_start is None else seq_start.data_ptr(),
+             128 ** -0.5 if scale is None else float(scale), int(causal)), (C.byref(od),))
+    return out
+
+
+def prompt_attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, *,
+                            scale: float | None = None, causal: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sequences laid end to end: ``query`` [total, Hq, 128], ``key`` / ``value`` [total, Hkv, 128] -> [total, Hq, 128].  Sequence
+    ``s`` is the tokens ``[cu_seqlens[s], cu_seqlens[s + 1])`` (int32 on the device, ascending) and attends itself alone;
+    none is longer than ``max_seqlen``.  Tokens behind the last sequence are left as they were in ``out``."""
+    _check(query, key, value, 3, 1)
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be an int32 tensor [sequences + 1]")
+    cu_seqlens = _int32(cu_seqlens, (int(cu_seqlens.numel()),), query.device, "cu_seqlens")
+    total, hq, hkv, n = int(query.shape[0]), int(query.shape[1]), int(key.shape[1]), int(cu_seqlens.numel()) - 1
+    if key.shape[0] != total or not 0 <= int(max_seqlen) <= total:
+        raise ValueError(f"{total} queries, {int(key.shape[0])} keys and sequences of up to {max_seqlen} tokens do not go together")
+    out = _output(out, query, lambda: torch.empty(total, hq, 128, dtype=query.dtype, device=query.device))
+    if n == 0 or max_seqlen == 0:
+        return out
+    q, k, v = aligned_view(query), aligned_view(key), aligned_view(value)
+    descs = [strided_desc(t.transpose(0, 1).unsqueeze(0)) for t in (q, k, v, out)]
+    refs = [C.byref(d) for d in descs]
+    _launch("tq_prompt_attn_packed", query.device, (n, hq, hkv, int(max_seqlen), int(max_seqlen)),
+            (refs[0], refs[1], refs[2], n, total, hq, hkv, cu_seqlens.data_ptr(), int(max_seqlen),
+             128 ** -0.5 if scale is None else float(scale), int(causal)), (refs[3],))
+    return out
+
+
+def raise_on_status(device: torch.device, where: str) -> None:
+    """Raise :class:`TQError` when a prompt kernel of this device has given up waiting (synchronises with the device)."""
+    v = C.c_int32()
+    with torch.cuda.device(device):
+        ffi.check(ffi.lib().tq_prompt_status(C.byref(v)), "tq_prompt_status")
+    if v.value:
+        raise ffi.TQError(f"{where}: a prompt attention kernel's wait ran out; its outputs are not valid")
+
+
+def _takes(query, key, attention_mask, is_causal, dropout, kwargs) -> bool:
+    """Whether the kernels compute what the model asks for here: causal attention of 16-bit tensors with 128 coordinates per head
+    and at most left padding."""
+    return (query.device.type == "cuda" and query.dtype in (torch.float16, torch.bfloat16) and key.dtype == query.dtype
+            and query.shape[-1] == 128 and key.shape[-1] == 128 and query.shape[2] <= key.shape[2] and is_causal and not dropout
+            and query.shape[1] // key.shape[1] <= 64
+            and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad))
+            and (attention_mask is None or attention_mask.dim() == 4)
+            and not any(kwargs.get(name) is not None for name in ("sliding_window", "softcap", "s_aux", "position_bias")))
+
+
+def turboquant_prompt_forward(module, query, key, value, attention_mask, dropout: float = 0.0, scaling: float | None = None,
+                              is_causal: bool | None = None, **kwargs):
+    """HF attention function of the prompt pass, ``(module, query[B,Hq,Sq,D], key, value, mask, ...) -> (out[B,Sq,Hq,D], None)``.  The
+    mask is that of a causal, at most left-padded batch (``generate`` switches here only for those); what the kernels do not compute
+    goes to ``F.scaled_dot_product_attention``."""
+    from tq_local_b200.runtime.attention import _sdpa_fallback
+    from tq_local_b200.runtime.packed_qmse_cache import leading_masked_tokens
+
+    causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
+    if not _takes(query, key, attention_mask, causal, dropout, kwargs):
+        return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
+    starts = None if attention_mask is None else leading_masked_tokens(attention_mask).expand(query.shape[0])
+    return prompt_attention(query, key, value, scale=scaling, seq_start=starts).transpose(1, 2), None
+
+
+def register_prompt_backend() -> None:
+    """Register ``"turboquant_prompt"`` with ``transformers`` (and the SDPA mask builder under the same key); idempotent."""
+    try:
+        from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+    except ImportError:
+        return
+    ALL_ATTENTION_FUNCTIONS.register("turboquant_prompt", turboquant_prompt_forward)
+    try:
+        from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
+
+        ALL_MASK_ATTENTION_FUNCTIONS.register("turboquant_prompt", ALL_MASK_ATTENTION_FUNCTIONS["sdpa"])
+    except (ImportError, KeyError):
+        pass

@@ -20,6 +20,7 @@ __all__ = list(_impl.__all__)
 _ALIASES = (
     "api", "constants", "telemetry", "quantization", "quantization.turboquant_mse", "runtime",
     "runtime.attention", "runtime.generation", "runtime.memory_accounting", "runtime.packed_qmse_cache",
+    "runtime.prompt_attention",
     "adapters", "adapters.transformers",
 )
 
