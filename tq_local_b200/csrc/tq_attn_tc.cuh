@@ -1,0 +1,97 @@
+// Pieces shared by the tcgen05 attention kernels: products with both operands in shared memory or A in TMEM, TMEM moves of 32 columns,
+// tensor-map copies, and the exponentials of a row.
+#pragma once
+
+#include "tq_umma.cuh"
+
+// Instruction descriptor: D = f32, A = B = f16 or bf16, A K-major, N = M = 128; NEGATE: -A.
+template <bool BF16, bool TRANSPOSED> __host__ __device__ constexpr uint32_t attn_instr(bool negate = false) {
+    return umma_instr<TRANSPOSED>() | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (negate ? 1u << 13 : 0u);
+}
+
+// D[128 x 128] (+)= A[128 x 16] * B, both in shared memory
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t instr, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(instr), "r"(accumulate)
+        : "memory");
+}
+
+// D[128 x 128] = A[128 x 128] * B^T, both row-major images of two 64-wide slabs (see umma_operand_offset).
+__device__ __forceinline__ void attn_scores(uint32_t d, uint32_t a_addr, uint32_t b_addr, uint32_t instr, uint32_t accumulate = 0) {
+    const uint64_t a = umma_desc<false>(a_addr), b = umma_desc<false>(b_addr);
+#pragma unroll
+    for (uint32_t s = 0; s < 8; ++s) {
+        const uint32_t step = ((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4;
+        umma_ss(d, a + step, b + step, instr, accumulate | (s > 0));
+    }
+}
+// D[128 x 128] (+)= P[128 x 128] * V, P as packed 16-bit pairs in TMEM, V a row-major image (rows are tokens).
+__device__ __forceinline__ void attn_values(uint32_t d, uint32_t p, uint32_t v_addr, uint32_t instr, uint32_t accumulate) {
+    const uint64_t b = umma_desc<true>(v_addr);
+#pragma unroll
+    for (uint32_t s = 0; s < 8; ++s) umma_f16(d, p + 8 * s, b + ((s * 16 * 128) >> 4), instr, accumulate | (s > 0));
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {  // tmem_ld_wait before they are used
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {  // tmem_st_wait before anybody reads them
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+// (the registers are named so that nothing reads them ahead of the wait)
+__device__ __forceinline__ void tmem_ld_wait(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_one(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+
+template <bool BF16> __device__ __forceinline__ uint32_t pack16(float a, float b) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float exp2_hw(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// The running maximum that a row's weights are relative to may lag behind the true one by up to 2^kLag: fp16 weights stay below
+// 2^9 and the sums far from overflow, and the accumulator is rescaled a few times a row instead of at every block.
+constexpr float kLag = 8.f;

@@ -1,59 +1,437 @@
-// Attention of a whole prompt over dense keys and values: out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys a query sees.
+// Attention of a whole prompt over dense keys and values on the 5th-generation tensor cores:
 //
-// One warp per (query, head): a pass over its keys with the running maximum and sum of the softmax, four coordinates a lane.
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the keys a query sees
+//
+// in one pass over the keys, 128 at a time, with the running maximum and sum of the softmax; logits and weights stay on the SM.
+//
+// Rows.  The query heads of a KV head share its keys, so a tile's 128 rows are (position, head of the group) pairs, positions
+// outermost: keys and values are read once for all of them, and a tile ends at its own last position, which leaves little of a
+// causal mask inside it.  A CTA owns two tiles (one, where tiles are few): while the tensor core multiplies for one, the other's
+// warps take exponentials.
+//
+// Roles.  Warps 0-3 and 4-7: the softmax of a tile each, one row a thread.  Warp 8: requests the query tiles and the key and value blocks
+// (tensor maps, 128-byte swizzle, a ring of 32 KB slots).  Warp 9: issues the products.  S = Q K^T with both operands in
+// shared memory; the weights go back to TMEM over S as 16-bit pairs and are the A operand of O += P V.
+// TMEM: S of the two tiles, O of the two tiles, 128 columns each.
+#include <cuda.h>
 #include <math.h>
 
-#include "tq_common.cuh"
+#include "tq_attn_tc.cuh"
 
 namespace {
 
 __device__ int g_prompt_status;
 
+constexpr int kThreads = 384;
+constexpr int kBlock = 128;                      // keys of a block
+constexpr int kSlotBytes = kUmmaTermBytes;       // 128 rows x 128 16-bit values
+constexpr int kSlots = 5;
+constexpr int kSmem = 2 * kSlotBytes + kSlots * kSlotBytes + 1024;
+
 struct PromptArgs {
-    const void *q, *k, *v;
     void *out;
-    int64_t qb, qh, qt, kb, kh, kt, vb, vh, vt, ob, oh, ot;
-    int q_heads, group, n_q, n_kv;
+    int64_t ob, oh, ot;
+    int batch, kv_heads, group, positions;  // positions of a tile: 128 / group
+    int n_q, n_kv, n_items, tiles_per_cta, splits;
     const int *seq_start, *cu_seqlens;
-    float scale;
-    bool causal;
+    float scale_log2;  // |scale| log2(e)
+    bool causal, negate;
+    float *part_ml, *part_o;  // splits > 1: [row][split] maximum (log2) and sum, [row][split][128]
 };
 
-template <typename T> __device__ __forceinline__ float4 load4(const void *base, int64_t at) {
-    const T *p = reinterpret_cast<const T *>(base) + at;
-    return make_float4(tq_to_float<T>(p[0]), tq_to_float<T>(p[1]), tq_to_float<T>(p[2]), tq_to_float<T>(p[3]));
+__device__ __forceinline__ void load_map(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w, int v) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];\n" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+                 : "memory");
+}
+__device__ __forceinline__ void load_map(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+                 : "memory");
 }
 
-template <typename T> __global__ void __launch_bounds__(128) tq_prompt_kernel(const __grid_constant__ PromptArgs a) {
-    const int lane = threadIdx.x & 31, i = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-    int64_t t0 = 0;
-    int n_q = a.n_q, n_kv = a.n_kv;
-    if (a.cu_seqlens) t0 = a.cu_seqlens[b], n_q = n_kv = min(a.cu_seqlens[b + 1] - (int)t0, a.n_q);
-    if (i >= n_q) return;
-    const int64_t bb = a.cu_seqlens ? 0 : b;
-    const float4 q = load4<T>(a.q, bb * a.qb + h * a.qh + (t0 + i) * a.qt + 4 * lane);
-    const int first = a.seq_start ? max(a.seq_start[b], 0) : 0, last = a.causal ? min(n_kv, i + n_kv - n_q + 1) : n_kv;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = first; j < last; ++j) {
-        const float4 k = load4<T>(a.k, bb * a.kb + h / a.group * a.kh + (t0 + j) * a.kt + 4 * lane);
-        const float4 v = load4<T>(a.v, bb * a.vb + h / a.group * a.vh + (t0 + j) * a.vt + 4 * lane);
-        const float s = a.scale * tq_warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w);
-        const float m_new = fmaxf(m, s), keep = m_new == -INFINITY ? 1.f : expf(m - m_new), p = m_new == -INFINITY ? 0.f : expf(s - m_new);
-        m = m_new, l = l * keep + p;
-        o = make_float4(o.x * keep + p * v.x, o.y * keep + p * v.y, o.z * keep + p * v.z, o.w * keep + p * v.w);
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    tq_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ PromptArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_bars[4 + 4 + 2 * kSlots];
+    __shared__ uint32_t s_tmem;
+    // ---- this CTA's work: the longest tiles come first
+    const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads % a.batch;
+    const int item = a.n_items - 1 - blockIdx.x / (a.kv_heads * a.batch);
+    int n_q = a.n_q, n_kv = a.n_kv, t0 = 0;
+    if (a.cu_seqlens) t0 = a.cu_seqlens[b], n_q = n_kv = min(a.cu_seqlens[b + 1] - t0, a.n_q);
+    const int first_pos = item * a.tiles_per_cta * a.positions;
+    if (first_pos >= n_q) return;
+    const int offset = n_kv - n_q;
+    const int start = a.seq_start ? min(max(a.seq_start[b], 0), n_kv) : 0;
+    const int block0 = start / kBlock;
+    auto blocks_of = [&](int w) {
+        const int pos = first_pos + w * a.positions;
+        if (w >= a.tiles_per_cta || pos >= n_q) return 0;
+        const int end = a.causal ? min(n_kv, min(pos + a.positions, n_q) + offset) : n_kv;
+        return end > start ? (end + kBlock - 1) / kBlock - block0 : 0;
+    };
+    int nb0 = blocks_of(0), nb1 = blocks_of(1);
+    int first_block = block0;
+    if (a.splits > 1) {
+        const int share = (max(nb0, nb1) + a.splits - 1) / a.splits, lo = share * blockIdx.y;
+        first_block += lo, nb0 = min(max(nb0 - lo, 0), share), nb1 = min(max(nb1 - lo, 0), share);
     }
-    const float inv = l > 0.f || isnan(l) ? 1.f / l : 0.f;
-    T *p = reinterpret_cast<T *>(a.out) + bb * a.ob + h * a.oh + (t0 + i) * a.ot + 4 * lane;
-    p[0] = tq_from_float<T>(o.x * inv), p[1] = tq_from_float<T>(o.y * inv), p[2] = tq_from_float<T>(o.z * inv), p[3] = tq_from_float<T>(o.w * inv);
+    const int nb = max(nb0, nb1);
+
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + 2 * kSlotBytes;
+    const uint32_t bars = smem_u32(s_bars);
+    const uint32_t bar_q = bars, bar_s = bars + 16, bar_p = bars + 32, bar_o = bars + 48, bar_full = bars + 64, bar_empty = bar_full + 8 * kSlots;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
+    if (tid == 0) {
+        mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1);
+        for (int w = 0; w < 2; ++w) mbar_init(bar_s + 8 * w, 1), mbar_init(bar_p + 8 * w, 128), mbar_init(bar_o + 8 * w, 1);
+        for (int s = 0; s < kSlots; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    }
+    umma_fence_before();
+    __syncthreads();
+    umma_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    bool lost = false;  // a wait of this thread ran out: it waits for nothing more
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!lost && !mbar_wait(bar, parity)) lost = true;
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+        if (warp == 8 && elect_one()) {
+            // ---------------- copies: Q0, K0, Q1, V0, K1, V1, ...
+            const int bb = a.cu_seqlens ? 0 : b;
+            auto load_q = [&](int w) {
+                mbar_expect_tx(bar_q + 8 * w, 256 * a.positions * a.group);
+                for (int x = 0; x < 2; ++x)
+                    load_map(base + w * kSlotBytes + x * kUmmaSlabBytes, &map_q, bar_q + 8 * w, 64 * x, 0, t0 + first_pos + w * a.positions, h, bb);
+            };
+            if (nb0) load_q(0);
+            for (int i = 0; i < 2 * nb; ++i) {
+                const int slot = i % kSlots;
+                wait(bar_empty + 8 * slot, (i / kSlots & 1) ^ 1);
+                const uint32_t bar = bar_full + 8 * slot;
+                mbar_expect_tx(bar, kSlotBytes);
+                for (int x = 0; x < 2; ++x)
+                    load_map(ring + slot * kSlotBytes + x * kUmmaSlabBytes, i & 1 ? &map_v : &map_k, bar, 64 * x, t0 + (first_block + i / 2) * kBlock, h, bb);
+                if (i == 0 && nb1) load_q(1);
+            }
+        } else if (warp == 9) {
+            // ---------------- products
+            const uint32_t instr_s = attn_instr<BF16, false>(a.negate), instr_o = attn_instr<BF16, true>();
+            auto slot_addr = [&](int i) { return ring + i % kSlots * kSlotBytes; };
+            auto wait_full = [&](int i) { wait(bar_full + 8 * (i % kSlots), i / kSlots & 1); };
+            auto scores = [&](int w, int i) {
+                if (elect_one()) {
+                    attn_scores(tmem + 128 * w, base + w * kSlotBytes, slot_addr(i), instr_s);
+                    umma_commit(bar_s + 8 * w);
+                }
+                __syncwarp();
+            };
+            if (nb) {
+                wait_full(0);
+                if (nb0) wait(bar_q, 0), umma_fence_after(), scores(0, 0);
+                if (nb1) wait(bar_q + 8, 0), umma_fence_after(), scores(1, 0);
+                if (kSlots < 2 * nb && elect_one()) umma_commit(bar_empty);
+                __syncwarp();
+            }
+            for (int k = 0; k < nb; ++k) {
+                const int iv = 2 * k + 1, ik = 2 * k + 2;
+                wait_full(iv);
+                // Values that no query sees may hold anything, and 0 * inf is not 0: they become 0.
+                const int j0 = (first_block + k) * kBlock, dirty_lo = start - j0, clean_hi = n_kv - j0;
+                if (dirty_lo > 0 || clean_hi < kBlock) {
+                    for (int i = tid & 31; i < kBlock * 16; i += 32) {
+                        const int row = i >> 4;
+                        if (row < dirty_lo || row >= clean_hi) sts128(slot_addr(iv) + (i & 8) / 8 * kUmmaSlabBytes + row * 128 + (i & 7) * 16, 0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    __syncwarp();
+                }
+                if (k + 1 < nb) wait_full(ik);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int mine = w ? nb1 : nb0;
+                    if (k >= mine) continue;
+                    wait(bar_p + 8 * w, k & 1);
+                    umma_fence_after();
+                    if (elect_one()) {
+                        attn_values(tmem + 256 + 128 * w, tmem + 128 * w, slot_addr(iv), instr_o, k > 0);
+                        if (k + 1 == mine) umma_commit(bar_o + 8 * w);
+                    }
+                    __syncwarp();
+                    if (k + 1 < mine) scores(w, ik);
+                }
+                if (iv + kSlots < 2 * nb && elect_one()) {  // (a slot that is filled again)
+                    umma_commit(bar_empty + 8 * (iv % kSlots));
+                    if (ik + kSlots < 2 * nb) umma_commit(bar_empty + 8 * (ik % kSlots));
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ---------------- softmax of tile w, one row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+        const int w = warp >> 2, row = tid & 127, mine = w ? nb1 : nb0;
+        const int pos = first_pos + w * a.positions + row / a.group;
+        const bool live = w < a.tiles_per_cta && row < a.positions * a.group && pos < n_q;
+        const int limit = a.causal ? min(n_kv, pos + offset + 1) : n_kv;  // keys [start, limit)
+        const int tile_limit = a.causal ? min(n_kv, first_pos + w * a.positions + offset + 1) : n_kv;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_s = tmem + 128 * w + lanes, t_o = tmem + 256 + 128 * w + lanes;
+        const float c = a.scale_log2;
+        float m_ref = -INFINITY;
+        uint64_t sum[2] = {0, 0};
+        for (int k = 0; k < mine; ++k) {
+            wait(bar_s + 8 * w, k & 1);
+            __syncwarp();
+            umma_fence_after();
+            uint32_t s[128];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s + 32 * i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_ld_wait(s + 32 * i);
+            const int j0 = (first_block + k) * kBlock;
+            if (j0 < start || j0 + kBlock > tile_limit) {
+                const int lo = start - j0, hi = limit - j0;
+#pragma unroll
+                for (int i = 0; i < 128; ++i)
+                    if (i < lo || i >= hi) s[i] = 0xff800000u;
+            }
+            float top[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i] = max3(__uint_as_float(s[i]), __uint_as_float(s[i + 4]), __uint_as_float(s[i + 8]));
+#pragma unroll
+            for (int i = 12; i < 124; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
+            float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            peak = fmaxf(peak, max3(__uint_as_float(s[124]), __uint_as_float(s[125]), fmaxf(__uint_as_float(s[126]), __uint_as_float(s[127]))));
+            if (k == 0) {
+                m_ref = peak;
+            } else {
+                const bool raise = live && (peak - m_ref) * c > kLag;
+                if (__any_sync(0xffffffffu, raise)) {
+                    float keep = 1.f;
+                    if (raise) keep = exp2_hw((m_ref - peak) * c), m_ref = peak;
+                    const uint64_t keep2 = f32x2(keep, keep);
+                    sum[0] = f32x2_mul(sum[0], keep2), sum[1] = f32x2_mul(sum[1], keep2);
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {  // (S_k was multiplied after O_(k-1): nobody else touches O now)
+                        uint32_t o[32];
+                        tmem_ld32(t_o + 32 * i, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_st32(t_o + 32 * i, o);
+                    }
+                }
+            }
+            const float shift = m_ref == -INFINITY ? 0.f : -m_ref * c;
+            const uint64_t c2 = f32x2(c, c), shift2 = f32x2(shift, shift);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float x, y;
+                    f32x2_split(f32x2_fma(f32x2(__uint_as_float(s[64 * half + 2 * i]), __uint_as_float(s[64 * half + 2 * i + 1])), c2, shift2), x, y);
+                    x = exp2_hw(x), y = exp2_hw(y);
+                    sum[i & 1] = f32x2_add(sum[i & 1], f32x2(x, y));
+                    p[i] = pack16<BF16>(x, y);
+                }
+                tmem_st32(t_s + 32 * half, p);
+            }
+            tmem_st_wait();
+            umma_fence_before();
+            mbar_arrive_one(bar_p + 8 * w);
+        }
+        // ---------------- the tile's rows
+        float l0, l1;
+        f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
+        const float l = l0 + l1;
+        if (mine) {
+            wait(bar_o + 8 * w, 0);
+            __syncwarp();
+            umma_fence_after();
+        }
+        const int head = h * a.group + row % a.group;
+        if (a.splits > 1) {
+            const int64_t r = (((int64_t)b * a.n_q + pos) * (a.kv_heads * a.group) + head) * a.splits + blockIdx.y;
+            if (live) a.part_ml[2 * r] = m_ref * c, a.part_ml[2 * r + 1] = l;
+            if (mine) {
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tmem_ld32(t_o + 32 * i, o);
+                    tmem_ld_wait(o);
+                    if (live)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(a.part_o + r * TQ_D + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+        } else {
+            uint8_t *dst = reinterpret_cast<uint8_t *>(a.out) + 2 * ((a.cu_seqlens ? 0 : b) * a.ob + head * a.oh + (int64_t)(t0 + pos) * a.ot);
+            const bool any = l > 0.f || l != l;
+            const float inv = any ? 1.f / l : 0.f;
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                uint32_t o[32] = {};
+                __syncwarp();
+                if (mine) {
+                    tmem_ld32(t_o + 32 * i, o);
+                    tmem_ld_wait(o);
+                }
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t r[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            r[x] = any ? pack16<BF16>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv) : 0u;
+                        *reinterpret_cast<uint4 *>(dst + 64 * i + 2 * e) = make_uint4(r[0], r[1], r[2], r[3]);
+                    }
+                }
+            }
+        }
+    }
+    if (lost) atomicExch(&g_prompt_status, 1);
+    umma_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        umma_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
+    }
+}
+
+// A row's partials from its splits: one warp a row.
+template <bool BF16> __global__ void __launch_bounds__(128) tq_prompt_join_kernel(const __grid_constant__ PromptArgs a, int64_t rows) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, heads = a.kv_heads * a.group;
+    if (r >= rows) return;
+    const int head = (int)(r % heads), pos = (int)(r / heads % a.n_q), b = (int)(r / heads / a.n_q);
+    int t0 = 0;
+    if (a.cu_seqlens) {
+        t0 = a.cu_seqlens[b];
+        if (pos >= min(a.cu_seqlens[b + 1] - t0, a.n_q)) return;
+    }
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + r * a.splits;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s].x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 part = ml[s];
+        if (part.y == 0.f) continue;  // (nothing of it was stored)
+        const float f = exp2f(part.x - m);
+        const float4 v = reinterpret_cast<const float4 *>(a.part_o + (r * a.splits + s) * TQ_D)[lane];
+        l += f * part.y;
+        o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    uint2 *dst = reinterpret_cast<uint2 *>(reinterpret_cast<uint8_t *>(a.out) + 2 * ((a.cu_seqlens ? 0 : b) * a.ob + head * a.oh + (int64_t)(t0 + pos) * a.ot)) + lane;
+    *dst = make_uint2(pack16<BF16>(o.x * inv, o.y * inv), pack16<BF16>(o.z * inv, o.w * inv));
 }
 
 bool aligned(const tq_dense_desc *d) {
     return !(((uintptr_t)d->data | (uintptr_t)(2 * (d->stride_b | d->stride_h | d->stride_t))) & 15);
 }
 
+int sm_count() {
+    int device = 0, n = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    return n;
+}
+
+// Two tiles a CTA as soon as one each would not fit the SMs at a time.  Where even those leave SMs idle, the keys are cut: a block of keys
+// takes a CTA about a microsecond and joining the pieces a launch, so a piece has at least four blocks.
+struct Plan {
+    int positions, tiles_per_cta, n_items, splits;
+};
+Plan plan(int64_t batch, int q_heads, int kv_heads, int n_q, int n_kv) {
+    Plan p;
+    p.positions = kUmmaRows / (q_heads / kv_heads);
+    const int sms = sm_count(), tiles = (n_q + p.positions - 1) / p.positions;
+    p.tiles_per_cta = batch * kv_heads * tiles > sms ? 2 : 1;
+    p.n_items = (tiles + p.tiles_per_cta - 1) / p.tiles_per_cta;
+    const int64_t ctas = batch * kv_heads * p.n_items;
+    const int blocks = (n_kv + kBlock - 1) / kBlock;
+    p.splits = ctas && ctas <= sms / 2 ? (int)(sms / ctas < blocks / 4 ? sms / ctas : blocks / 4) : 1;
+    if (p.splits < 1) p.splits = 1;
+    return p;
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                             const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// A map of a 16-bit tensor of 128 coordinates with `dims - 1` outer axes, copied in boxes of 64 coordinates.
+bool encode(CUtensorMap *map, bool bf16, const void *data, int dims, const int64_t *sizes, const int64_t *strides, const int *box) {
+    cuuint64_t size[5] = {TQ_D}, stride[4];
+    cuuint32_t boxes[5] = {64}, steps[5] = {1, 1, 1, 1, 1};
+    for (int i = 1; i < dims; ++i) {
+        size[i] = (cuuint64_t)sizes[i - 1], boxes[i] = (cuuint32_t)box[i - 1];
+        stride[i - 1] = sizes[i - 1] > 1 ? (cuuint64_t)strides[i - 1] * 2 : 2 * TQ_D;  // (an axis of one element has no stride of its own)
+    }
+    const EncodeFn fn = encode_fn();
+    return fn && fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void *>(data), size, stride, boxes, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16> int32_t launch(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int64_t tokens_q, int64_t tokens_kv, int maps_batch,
+                                    const PromptArgs &a, cudaStream_t stream) {
+    CUtensorMap maps[3];
+    const int64_t q_sizes[4] = {a.group, tokens_q, a.kv_heads, maps_batch}, q_strides[4] = {q->stride_h, q->stride_t, q->stride_h * a.group, q->stride_b};
+    const int q_box[4] = {a.group, a.positions, 1, 1}, kv_box[3] = {kBlock, 1, 1};
+    bool ok = encode(&maps[0], BF16, q->data, 5, q_sizes, q_strides, q_box);
+    const tq_dense_desc *kv[2] = {k, v};
+    for (int i = 0; i < 2; ++i) {
+        const int64_t sizes[3] = {tokens_kv, a.kv_heads, maps_batch}, strides[3] = {kv[i]->stride_t, kv[i]->stride_h, kv[i]->stride_b};
+        ok = ok && encode(&maps[1 + i], BF16, kv[i]->data, 4, sizes, strides, kv_box);
+    }
+    if (!ok) {
+        tq_set_cuda_error(cudaErrorInvalidValue, "tensor map of a prompt's queries, keys or values");
+        return TQ_ERR_CUDA;
+    }
+    int device = 0;
+    TQ_CUDA_CHECK(cudaGetDevice(&device));
+    TQ_CUDA_CHECK(tq_allow_shared<tq_prompt_kernel<BF16>>(device, kSmem));
+    const dim3 grid((unsigned)(a.batch * a.kv_heads * a.n_items), (unsigned)a.splits);
+    tq_prompt_kernel<BF16><<<grid, kThreads, kSmem, stream>>>(maps[0], maps[1], maps[2], a);
+    TQ_CUDA_CHECK(cudaGetLastError());
+    if (a.splits > 1) {
+        const int64_t rows = (int64_t)a.batch * a.n_q * a.kv_heads * a.group;
+        tq_prompt_join_kernel<BF16><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a, rows);
+        TQ_CUDA_CHECK(cudaGetLastError());
+    }
+    return TQ_OK;
+}
+
 int32_t prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int32_t batch, int32_t q_heads,
-                    int32_t kv_heads, int32_t n_q, int32_t n_kv, const int32_t *seq_start, const int32_t *cu_seqlens, float scale,
+                    int32_t kv_heads, int32_t n_q, int32_t n_kv, const int32_t *seq_start, const int32_t *cu_seqlens, int32_t total, float scale,
                     int32_t causal, void *workspace, size_t workspace_bytes, const tq_dense_desc *out, cudaStream_t stream) {
     if (!q || !k || !v || !out || !q->data || !k->data || !v->data || !out->data) return TQ_ERR_ARG;
     if (q->dtype != TQ_DTYPE_F16 && q->dtype != TQ_DTYPE_BF16) return q->dtype == TQ_DTYPE_F32 ? TQ_ERR_UNSUPPORTED : TQ_ERR_ARG;
@@ -62,31 +440,41 @@ int32_t prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_den
     if (q_heads / kv_heads > TQ_MAX_PROMPT_GROUPS) return TQ_ERR_UNSUPPORTED;
     if (causal && n_kv < n_q) return TQ_ERR_ARG;
     if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out)) return TQ_ERR_ARG;
-    if (((uintptr_t)seq_start | (uintptr_t)cu_seqlens) & 3) return TQ_ERR_ARG;
-    if (workspace_bytes < tq_prompt_workspace_bytes(batch, q_heads, kv_heads, n_q, n_kv)) return TQ_ERR_WORKSPACE;
+    if (((uintptr_t)seq_start | (uintptr_t)cu_seqlens) & 3 || (uintptr_t)workspace & 15) return TQ_ERR_ARG;
+    const size_t need = tq_prompt_workspace_bytes(batch, q_heads, kv_heads, n_q, n_kv);
+    if (workspace_bytes < need || (need && !workspace)) return TQ_ERR_WORKSPACE;
     if (batch == 0 || n_q == 0) return TQ_OK;
+    if (n_kv == 0 || !(fabsf(scale) <= 3.4e38f)) return TQ_ERR_ARG;
+    const Plan p = plan(batch, q_heads, kv_heads, n_q, n_kv);
+    if ((int64_t)batch * kv_heads * p.n_items > 0x7fffffff) return TQ_ERR_UNSUPPORTED;
     PromptArgs a = {};
-    a.q = q->data, a.k = k->data, a.v = v->data, a.out = const_cast<void *>(out->data);
-    a.qb = q->stride_b, a.qh = q->stride_h, a.qt = q->stride_t, a.kb = k->stride_b, a.kh = k->stride_h, a.kt = k->stride_t;
-    a.vb = v->stride_b, a.vh = v->stride_h, a.vt = v->stride_t, a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
-    a.q_heads = q_heads, a.group = q_heads / kv_heads, a.n_q = n_q, a.n_kv = n_kv, a.seq_start = seq_start, a.cu_seqlens = cu_seqlens;
-    a.scale = scale, a.causal = causal != 0;
-    const dim3 grid((n_q + 3) / 4, q_heads, batch);
-    if (q->dtype == TQ_DTYPE_F16) tq_prompt_kernel<__half><<<grid, 128, 0, stream>>>(a);
-    else tq_prompt_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(a);
-    TQ_CUDA_CHECK(cudaGetLastError());
-    return TQ_OK;
+    a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
+    a.batch = batch, a.kv_heads = kv_heads, a.group = q_heads / kv_heads, a.positions = p.positions;
+    a.n_q = n_q, a.n_kv = n_kv, a.n_items = p.n_items, a.tiles_per_cta = p.tiles_per_cta, a.splits = p.splits;
+    a.seq_start = seq_start, a.cu_seqlens = cu_seqlens, a.causal = causal != 0, a.negate = scale < 0.f;
+    a.scale_log2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);  // (not 0: a masked logit is -inf and has to stay so)
+    if (p.splits > 1) {
+        const size_t rows = (size_t)batch * n_q * q_heads * p.splits;
+        a.part_o = static_cast<float *>(workspace), a.part_ml = a.part_o + rows * TQ_D;
+    }
+    const int64_t tokens_q = cu_seqlens ? total : n_q, tokens_kv = cu_seqlens ? total : n_kv;
+    return q->dtype == TQ_DTYPE_BF16 ? launch<true>(q, k, v, tokens_q, tokens_kv, cu_seqlens ? 1 : batch, a, stream)
+                                     : launch<false>(q, k, v, tokens_q, tokens_kv, cu_seqlens ? 1 : batch, a, stream);
 }
 
 }  // namespace
 
-extern "C" size_t tq_prompt_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv) { return 0; }
+extern "C" size_t tq_prompt_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv) {
+    if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads / kv_heads > kUmmaRows || n_q <= 0 || n_kv <= 0) return 0;
+    const Plan p = plan(batch, q_heads, kv_heads, n_q, n_kv);
+    return p.splits > 1 ? (size_t)batch * n_q * q_heads * p.splits * (TQ_D + 2) * sizeof(float) : 0;
+}
 
 extern "C" int32_t tq_prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int32_t batch, int32_t q_heads,
                                   int32_t kv_heads, int32_t n_q, int32_t n_kv, const int32_t *seq_start, float scale, int32_t causal,
                                   void *workspace, size_t workspace_bytes, const tq_dense_desc *out, tq_stream stream) {
     TqRange range_("tq_prompt_attn");
-    return prompt_attn(q, k, v, batch, q_heads, kv_heads, n_q, n_kv, seq_start, nullptr, scale, causal, workspace, workspace_bytes, out,
+    return prompt_attn(q, k, v, batch, q_heads, kv_heads, n_q, n_kv, seq_start, nullptr, 0, scale, causal, workspace, workspace_bytes, out,
                        (cudaStream_t)stream);
 }
 
@@ -95,8 +483,8 @@ extern "C" int32_t tq_prompt_attn_packed(const tq_dense_desc *q, const tq_dense_
                                          float scale, int32_t causal, void *workspace, size_t workspace_bytes, const tq_dense_desc *out,
                                          tq_stream stream) {
     TqRange range_("tq_prompt_attn_packed");
-    if (!cu_seqlens || total < 0 || max_seqlen < 0) return TQ_ERR_ARG;
-    return prompt_attn(q, k, v, n_seqs, q_heads, kv_heads, max_seqlen, max_seqlen, nullptr, cu_seqlens, scale, causal, workspace,
+    if (!cu_seqlens || total < 0 || max_seqlen < 0 || (total == 0 && max_seqlen > 0 && n_seqs > 0)) return TQ_ERR_ARG;
+    return prompt_attn(q, k, v, n_seqs, q_heads, kv_heads, max_seqlen, max_seqlen, nullptr, cu_seqlens, total, scale, causal, workspace,
                        workspace_bytes, out, (cudaStream_t)stream);
 }
 
