@@ -156,6 +156,7 @@ def test_rows_that_see_nothing_and_odd_masks():
     out = store.tree_attn(q, words(mask), lengths=lengths)
     check(out, reference(store, q, 200, mask, lengths))
     assert (out[0, :, 3] == 0).all()
+    assert torch.equal(store.tree_attn(q, words(mask) | -1 << t, lengths=lengths), out)  # bits of nodes that do not exist
     store.set_seq_start(torch.tensor([0, 200], dtype=torch.int32, device="cuda"))
     none = torch.zeros(2, t, dtype=torch.int64, device="cuda")
     assert (store.tree_attn(q, none, lengths=lengths) == 0).all()

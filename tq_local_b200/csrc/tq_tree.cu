@@ -1,90 +1,611 @@
-// Attention of drafted tokens over the packed cache.  The T drafted tokens of every batch entry are packed at tokens
-// [tree_start, tree_start + T); node i attends the entry's history [seq_start, length) and the drafted tokens that its mask names:
+// Attention of drafted tokens over the packed cache, on the 5th-generation tensor cores.  The T drafted tokens of every batch entry are
+// packed at tokens [tree_start, tree_start + T); node i attends the entry's history [seq_start, length) and the drafted tokens that its
+// mask names:
 //
 //   logit_ij = scale (kn_j c_k[codes_j] . (R_k q_i) + rn_j sqrt(pi/2)/D signs_j . (S q_i)),   out_i = R_v^T sum_j p_ij vn_j c_v[codes_j]
 //
-// One warp per (node, head): a pass over its tokens with the running maximum and sum of the softmax, four coordinates a lane.
+// Three launches.  The first rotates and projects the queries, rounds them to fp16 (the scale to base 2 and the sketch's factor folded in)
+// and sums up how many blocks of 128 tokens the batch entries have.  The second attends: the 128 rows of a tile are (node, head of the group)
+// pairs, its blocks are those of history and drafted tokens laid end to end, and all tiles' blocks laid end to end are cut into
+// equal pieces, one a CTA (one CTA an SM).  The third joins a tile's pieces, un-rotates and rounds.
+//
+// Roles of the second: warps 4-11 turn packed tokens into fp16 operands in shared memory, two threads a token: centres times norm by a
+// table of centre pairs in shared memory, +-rn for the signs.  Warp 12 issues the products, S = [Rq | Sq] [K | signs]^T with the queries in TMEM
+// and O += P V.  Warps 0-3 take the softmax, a row a thread; the weights go back over S as 16-bit pairs.
+// TMEM: S of two blocks, O, the queries, 128 columns each.
 #include <math.h>
 
-#include "tq_common.cuh"
+#include "tq_attn_tc.cuh"
 
 namespace {
+
+constexpr int kThreads = 512;
+constexpr int kBlock = 128;  // tokens of a block
+constexpr int kPrepRows = 16;
 
 struct TreeArgs {
     const uint8_t *k_codes, *k_signs, *v_codes;
     const uint16_t *k_norms, *k_rnorms, *v_norms;
     int64_t cache_sb, cache_sh;
-    int key_bits, bits, use_qjl, kv_heads, group, nodes, tree_start;
+    int batch, kv_heads, group, nodes, tree_start;
+    int positions, tiles, rows;  // nodes of a tile, tiles of a (batch entry, KV head), rows of a tile that hold something
     const int *seq_start, *lengths;
     const uint64_t *mask;
     const float *rot_k_t, *rot_v, *qjl_t, *centers_k, *centers_v;
     const void *q;
     void *out;
     int64_t qb, qh, qt, ob, oh, ot;
+    int64_t *prefix;  // [batch + 1] blocks of the entries before
+    uint16_t *qop;    // [batch][kv_heads][tiles][rows][128 or 256] fp16
+    float *part_ml, *part_o;  // [piece][rows][2], [piece][rows][128]
+    int ctas;
+    int *error_flag;
 };
 
-__device__ __forceinline__ int code_at(const uint8_t *p, int bits, int e) {
-    const int bit = e * bits, byte = bit >> 3, sh = bit & 7;
-    int w = p[byte];
-    if (sh + bits > 8) w |= p[byte + 1] << 8;
-    return (w >> sh) & ((1 << bits) - 1);
+struct Entry {
+    int start, history;
+};
+__device__ __forceinline__ Entry entry_of(const TreeArgs &a, int b) {
+    const int length = a.lengths ? min(max(a.lengths[b], 0), a.tree_start) : a.tree_start;
+    const int start = a.seq_start ? min(max(a.seq_start[b], 0), length) : 0;
+    return {start, length - start};
+}
+// tokens that tile t of an entry may see, in blocks
+__device__ __forceinline__ int tile_blocks(const TreeArgs &a, int history, int t) {
+    const int drafted = a.mask ? a.nodes : min(a.nodes, (t + 1) * a.positions);
+    return (history + drafted + kBlock - 1) / kBlock;
+}
+__device__ __forceinline__ int head_blocks(const TreeArgs &a, int history) {
+    int n = 0;
+    for (int t = 0; t < a.tiles; ++t) n += tile_blocks(a, history, t);
+    return n;
 }
 
-template <typename T> __global__ void __launch_bounds__(128) tq_tree_kernel(const __grid_constant__ TreeArgs a) {
-    __shared__ float s_vec[4][TQ_D];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.x * 4 + w, hq = blockIdx.y, b = blockIdx.z;
-    if (i >= a.nodes) return;
-    const T *q = reinterpret_cast<const T *>(a.q) + b * a.qb + hq * a.qh + i * a.qt;
-    for (int e = 0; e < 4; ++e) s_vec[w][4 * lane + e] = tq_to_float<T>(q[4 * lane + e]);
-    __syncwarp();
-    float qr[4] = {}, qp[4] = {};
-    for (int d = 0; d < TQ_D; ++d)
-        for (int e = 0; e < 4; ++e) {
-            qr[e] += a.rot_k_t[d * TQ_D + 4 * lane + e] * s_vec[w][d];
-            if (a.use_qjl) qp[e] += a.qjl_t[d * TQ_D + 4 * lane + e] * s_vec[w][d];
+// ---------------------------------------------------------------------------------------------------- queries
+// Operand rows [Rq | Sq], kPrepRows rows a block, a coordinate a thread.  Sketch coordinates lie in the order in which
+// the operand's signs do: (i, i + 16) side by side, see sign_pair.
+template <typename T, bool QJL> __global__ void __launch_bounds__(QJL ? 256 : 128) tq_tree_prep_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows) {
+    constexpr int kWide = QJL ? 256 : 128;
+    __shared__ float s_q[kPrepRows][TQ_D];
+    if (blockIdx.x == 0 && threadIdx.x < 32) {
+        int64_t before = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            const int b = b0 + threadIdx.x;
+            int64_t n = b < a.batch ? (int64_t)head_blocks(a, entry_of(a, b).history) * a.kv_heads : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t x = __shfl_up_sync(0xffffffffu, n, o);
+                if (threadIdx.x >= o) n += x;
+            }
+            if (b < a.batch) a.prefix[b + 1] = before + n;
+            before += __shfl_sync(0xffffffffu, n, 31);
         }
-    const int64_t row = b * a.cache_sb + hq / a.group * a.cache_sh;
-    const int first = a.seq_start ? max(a.seq_start[b], 0) : 0;
-    const int length = a.lengths ? min(max(a.lengths[b], 0), a.tree_start) : a.tree_start;
-    const uint64_t seen = a.mask ? a.mask[(int64_t)b * a.nodes + i] : 0;
-    float m = -INFINITY, l = 0.f, o[4] = {};
-    const float scale = 0.08838834764831845f, sketch = 1.2533141373155003f / (float)TQ_D;
-    for (int j = min(first, length); j < length + a.nodes; ++j) {
-        const int node = j - length;
-        if (node >= 0 && !(a.mask ? seen >> node & 1 : node <= i)) continue;
-        const int64_t t = row + (node < 0 ? j : a.tree_start + node);
-        float s = 0.f, x = 0.f;
-        for (int e = 0; e < 4; ++e) {
-            s += qr[e] * a.centers_k[code_at(a.k_codes + t * 16 * a.key_bits, a.key_bits, 4 * lane + e)];
-            if (a.use_qjl) x += code_at(a.k_signs + t * 16, 1, 4 * lane + e) ? qp[e] : -qp[e];
-        }
-        s *= tq_half_bits_to_float(a.k_norms[t]);
-        if (a.use_qjl) s += x * sketch * tq_half_bits_to_float(a.k_rnorms[t]);
-        s = scale * tq_warp_sum(s);
-        const float m_new = fmaxf(m, s), keep = m_new == -INFINITY ? 1.f : expf(m - m_new), p = m_new == -INFINITY ? 0.f : expf(s - m_new);
-        m = m_new, l = l * keep + p;
-        const float pv = p * tq_half_bits_to_float(a.v_norms[t]);
-        for (int e = 0; e < 4; ++e) o[e] = o[e] * keep + pv * a.centers_v[code_at(a.v_codes + t * 16 * a.bits, a.bits, 4 * lane + e)];
+        if (threadIdx.x == 0) a.prefix[0] = 0;
     }
-    const float inv = l > 0.f || isnan(l) ? 1.f / l : 0.f;
-    __syncwarp();
-    for (int e = 0; e < 4; ++e) s_vec[w][4 * lane + e] = o[e] * inv;
-    __syncwarp();
-    float y[4] = {};
-    for (int d = 0; d < TQ_D; ++d)
-        for (int e = 0; e < 4; ++e) y[e] += s_vec[w][d] * a.rot_v[d * TQ_D + 4 * lane + e];
-    T *out = reinterpret_cast<T *>(a.out) + b * a.ob + hq * a.oh + i * a.ot;
-    for (int e = 0; e < 4; ++e) out[4 * lane + e] = tq_from_float<T>(y[e]);
+    const int64_t row0 = (int64_t)blockIdx.x * kPrepRows;
+    const float scale = 0.08838834764831845f * 1.4426950408889634f;
+    for (int i = threadIdx.x; i < kPrepRows * TQ_D; i += kWide) {
+        const int64_t r = row0 + i / TQ_D;
+        float x = 0.f;
+        if (r < n_rows) {
+            const int in = (int)(r % a.rows);
+            const int64_t tile = r / a.rows;
+            const int t = (int)(tile % a.tiles), h = (int)(tile / a.tiles % a.kv_heads), b = (int)(tile / a.tiles / a.kv_heads);
+            const int node = t * a.positions + in / a.group;
+            if (node < a.nodes)
+                x = tq_to_float<T>(reinterpret_cast<const T *>(a.q)[b * a.qb + (h * a.group + in % a.group) * a.qh + node * a.qt + i % TQ_D]) * scale;
+        }
+        s_q[i / TQ_D][i % TQ_D] = x;
+    }
+    __syncthreads();
+    const int c = threadIdx.x & 127;
+    const bool sketch = threadIdx.x >= 128;
+    const int from = sketch ? (c & ~31) + (c & 1) * 16 + ((c & 31) >> 1) : c;  // the coordinate at place c
+    const float *m = (sketch ? a.qjl_t : a.rot_k_t) + from;
+    float acc[kPrepRows] = {};
+    for (int d = 0; d < TQ_D; d += 4) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __ldg(m + (d + e) * TQ_D);
+#pragma unroll
+        for (int r = 0; r < kPrepRows; ++r) {
+            const float4 x = *reinterpret_cast<const float4 *>(&s_q[r][d]);
+            acc[r] += x.x * w[0] + x.y * w[1] + x.z * w[2] + x.w * w[3];
+        }
+    }
+    const float f = sketch ? 1.2533141373155003f / (float)TQ_D : 1.f;
+#pragma unroll
+    for (int r = 0; r < kPrepRows; ++r)
+        if (row0 + r < n_rows) a.qop[(row0 + r) * kWide + threadIdx.x] = tq_float_to_half_bits(acc[r] * f);
+}
+
+// ---------------------------------------------------------------------------------------------------- attention
+template <int KB, int VB, bool QJL> struct Layout {
+    static constexpr int kStage = (QJL ? 3 : 2) * kUmmaTermBytes;  // keys, values, signs of a block
+    // A slot of a table holds one pair of centres once per lane, so that lanes read their own banks; half as often where 256 slots and
+    // two stages with signs leave no room (two lanes then share a bank).
+    static constexpr int kKeySlot = 128, kValueSlot = QJL && VB == 4 ? 64 : 128;
+    static constexpr int kKeyTable = (1 << 2 * KB) * kKeySlot, kValueTable = (1 << 2 * VB) * kValueSlot;
+    static constexpr int kBytes = 2 * kStage + kKeyTable + kValueTable + 1024;
+};
+
+// Word i of the operand from 32 codes in BITS words (and one that is not looked at): two neighbouring codes by one look-up, times the norm.
+template <int BITS, int SLOT> __device__ __forceinline__ uint32_t centre_pair(const uint32_t *words, int i, uint32_t lane_addr, uint32_t norm2) {
+    constexpr int kShift = SLOT == 128 ? 7 : 6;
+    constexpr uint32_t kMask = ((1u << 2 * BITS) - 1u) << kShift;
+    const int bit = 2 * BITS * i, w = bit >> 5, sh = bit & 31;
+    uint32_t x;
+    if (sh + 2 * BITS > 32) x = __funnelshift_r(words[w], words[w + 1], sh) << kShift;
+    else x = sh >= kShift ? words[w] >> (sh - kShift) : words[w] << (kShift - sh);
+    uint32_t v;
+    asm("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"((x & kMask) + lane_addr));
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&norm2));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// Bits [base, base + 32) of what a row sees, base relative to the first drafted token: all of the history, then the mask.
+__device__ __forceinline__ uint32_t seen_word(uint64_t mask, int chain_end, int base) {
+    uint32_t r = 0;
+    if (base < 0) r = base <= -32 ? 0xffffffffu : (1u << -base) - 1u;
+    if (chain_end >= 0) {  // a chain: nodes [0, chain_end)
+        const int n = chain_end - base;
+        return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : r | ((1u << n) - 1u);
+    }
+    if (base <= -32 || base >= 64) return r;
+    return r | (uint32_t)(base < 0 ? mask << -base : mask >> base);
+}
+
+template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 1) tq_tree_kernel(const __grid_constant__ TreeArgs a) {
+    using L = Layout<KB, VB, QJL>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 2 + 2 + 1 + 1];
+    __shared__ uint32_t s_tmem;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t table_k = base + 2 * L::kStage, table_v = table_k + L::kKeyTable;
+    const uint32_t bars = smem_u32(s_bars);
+    // full: operands are there; free: the products that read them are done; s: logits are there; p: weights are there; o: O += P V is done; q: queries are there
+    const uint32_t bar_kfull = bars, bar_vfull = bars + 16, bar_kfree = bars + 32, bar_vfree = bars + 48, bar_s = bars + 64, bar_p = bars + 80, bar_o = bars + 96, bar_q = bars + 104;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_kfull + 8 * i, 256), mbar_init(bar_vfull + 8 * i, 256);
+            mbar_init(bar_kfree + 8 * i, 1), mbar_init(bar_vfree + 8 * i, 1);
+            mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 128);
+        }
+        mbar_init(bar_o, 1), mbar_init(bar_q, 128);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    {
+        auto fill = [&](uint32_t table, int bytes, int slot, int bits, const float *centers) {
+            const int copies = slot / 4;
+            for (int i = tid; i < bytes / 4; i += kThreads) {
+                const int e = i / copies;
+                asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(table + 4 * i), "r"(half2_bits(centers[e & ((1 << bits) - 1)], centers[e >> bits])) : "memory");
+            }
+        };
+        fill(table_k, L::kKeyTable, L::kKeySlot, KB, a.centers_k);
+        fill(table_v, L::kValueTable, L::kValueSlot, VB, a.centers_v);
+    }
+    umma_fence_before();
+    __syncthreads();
+    umma_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), t_o = tmem + 256, t_q = tmem + 384;
+
+    // ---- this CTA's blocks: [flat, flat_end) of all tiles' blocks laid end to end
+    const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
+    int64_t flat = (int64_t)blockIdx.x * chunk;
+    const int64_t flat_end = min(flat + chunk, total);
+    struct Segment {  // the part of one tile inside this CTA's piece: blocks [k, k_end)
+        int b, h, t, history, start, k, k_end;
+        int64_t tile;
+    };
+    int b_at = 0;
+    if (flat < flat_end) {
+        int hi = a.batch;  // the entry that holds block `flat`
+        while (hi - b_at > 1) {
+            const int mid = (b_at + hi) >> 1;
+            if (a.prefix[mid] <= flat) b_at = mid;
+            else hi = mid;
+        }
+    }
+    int64_t b_first = flat < flat_end ? a.prefix[b_at] : 0, b_next = flat < flat_end ? a.prefix[b_at + 1] : 0;
+    auto next_segment = [&]() {
+        while (flat >= b_next) ++b_at, b_first = b_next, b_next = a.prefix[b_at + 1];
+        Segment g;
+        const Entry e = entry_of(a, b_at);
+        const int per_head = head_blocks(a, e.history);
+        int in = (int)(flat - b_first);
+        g.b = b_at, g.h = in / per_head, in -= g.h * per_head, g.start = e.start, g.history = e.history;
+        int nb = tile_blocks(a, e.history, 0);
+        for (g.t = 0; in >= nb;) in -= nb, ++g.t, nb = tile_blocks(a, e.history, g.t);
+        g.k = in;
+        const int64_t left = flat_end - flat;
+        g.k_end = left < nb - in ? in + (int)left : nb;
+        g.tile = ((int64_t)g.b * a.kv_heads + g.h) * a.tiles + g.t;
+        flat += g.k_end - g.k;
+        return g;
+    };
+    bool lost = false;  // a wait of this thread ran out: it waits for nothing more
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!lost && !mbar_wait(bar, parity)) lost = true;
+    };
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
+        if (warp == 12) {
+            // ---------------- products; n counts blocks since the kernel began
+            constexpr uint32_t instr_s = umma_instr<false>(), instr_o = umma_instr<true>();
+            auto scores = [&](uint32_t n) {
+                wait(bar_kfull + 8 * (n & 1), n >> 1 & 1);
+                umma_fence_after();
+                if (elect_one()) {
+                    const uint32_t stage = base + (n & 1) * L::kStage, d = tmem + 128 * (n & 1);
+#pragma unroll
+                    for (int part = 0; part < (QJL ? 2 : 1); ++part) {
+                        const uint64_t desc = umma_desc<false>(stage + 2 * part * kUmmaTermBytes);
+#pragma unroll
+                        for (uint32_t s = 0; s < 8; ++s)
+                            umma_f16(d, t_q + 64 * part + 8 * s, desc + (((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4), instr_s, part | (s > 0));
+                    }
+                    umma_commit(bar_s + 8 * (n & 1));
+                    umma_commit(bar_kfree + 8 * (n & 1));
+                }
+                __syncwarp();
+            };
+            uint32_t n = 0, segment = 0;
+            while (flat < flat_end) {
+                const Segment g = next_segment();
+                const uint32_t end = n + (g.k_end - g.k);
+                wait(bar_q, segment++ & 1);
+                scores(n);
+                for (bool first = true; n < end; ++n, first = false) {
+                    if (n + 1 < end) scores(n + 1);
+                    wait(bar_vfull + 8 * (n & 1), n >> 1 & 1);
+                    wait(bar_p + 8 * (n & 1), n >> 1 & 1);
+                    umma_fence_after();
+                    if (elect_one()) {
+                        attn_values(t_o, tmem + 128 * (n & 1), base + (n & 1) * L::kStage + kUmmaTermBytes, instr_o, !first);
+                        umma_commit(bar_vfree + 8 * (n & 1));
+                        umma_commit(bar_o);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------- operands: half of a token's coordinates a thread
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
+        const int row = tid & 127, half = (tid - 128) >> 7;
+        uint32_t kw[2 * KB + 1], vw[2 * VB + 1], sw[2];
+        uint16_t kn, vn, rn;
+        kw[2 * KB] = vw[2 * VB] = 0;
+        Segment g;
+        int k = 0, k_end = 0;
+        auto words = [&](const uint8_t *src, int n, uint32_t *w) {
+            if (n % 4 == 0) {
+                for (int i = 0; i < n; i += 4) {
+                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(src) + i / 4);
+                    w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+                }
+            } else {
+                for (int i = 0; i < n; i += 2) {
+                    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(src) + i / 2);
+                    w[i] = x.x, w[i + 1] = x.y;
+                }
+            }
+        };
+        auto fetch = [&]() {  // the next block's token of this thread; false behind the last
+            if (k == k_end) {
+                if (flat >= flat_end) return false;
+                g = next_segment(), k = g.k, k_end = g.k_end;
+            }
+            const int v = k * kBlock + row;
+            ++k;
+            kn = vn = rn = 0;
+            if (v < g.history + a.nodes) {
+                const int64_t t = g.b * a.cache_sb + g.h * a.cache_sh + (v < g.history ? g.start + v : a.tree_start + v - g.history);
+                words(a.k_codes + t * 16 * KB + 8 * KB * half, 2 * KB, kw);
+                words(a.v_codes + t * 16 * VB + 8 * VB * half, 2 * VB, vw);
+                kn = __ldg(a.k_norms + t), vn = __ldg(a.v_norms + t);
+                if (QJL) words(a.k_signs + t * 16 + 8 * half, 2, sw), rn = __ldg(a.k_rnorms + t);
+            }
+            return true;
+        };
+        const uint32_t lane_k = table_k + 4 * (lane & (L::kKeySlot / 4 - 1)), lane_v = table_v + 4 * (lane & (L::kValueSlot / 4 - 1));
+        const uint32_t my_row = base + half * kUmmaSlabBytes + (row >> 3) * 1024 + (row & 7) * 128, turn = row & 7;
+        for (int i = 0; i < 2 * KB; ++i) kw[i] = 0;
+        for (int i = 0; i < 2 * VB; ++i) vw[i] = 0;
+        sw[0] = sw[1] = 0;
+        bool more = fetch();
+        for (uint32_t n = 0; more; ++n) {
+            const uint32_t dst = my_row + (n & 1) * L::kStage, parity = (n >> 1 & 1) ^ 1;
+            wait(bar_kfree + 8 * (n & 1), parity);
+            const uint32_t kn2 = kn * 0x10001u, vn2 = vn * 0x10001u, rn2 = (rn * 0x10001u) ^ 0x80008000u;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = centre_pair<KB, L::kKeySlot>(kw, 4 * c + i, lane_k, kn2);
+                sts128(dst + ((c ^ turn) << 4), o[0], o[1], o[2], o[3]);
+            }
+            if (QJL) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {  // signs p and p + 16 of a word; a set bit is +
+                        const int p = (c & 3) * 4 + i;
+                        o[i] = ((sw[c >> 2] << (15 - p)) & 0x80008000u) ^ rn2;
+                    }
+                    sts128(dst + 2 * kUmmaTermBytes + ((c ^ turn) << 4), o[0], o[1], o[2], o[3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            mbar_arrive_one(bar_kfull + 8 * (n & 1));
+            uint32_t vnow[2 * VB + 1];
+#pragma unroll
+            for (int i = 0; i <= 2 * VB; ++i) vnow[i] = vw[i];
+            more = fetch();
+            wait(bar_vfree + 8 * (n & 1), parity);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = centre_pair<VB, L::kValueSlot>(vnow, 4 * c + i, lane_v, vn2);
+                sts128(dst + kUmmaTermBytes + ((c ^ turn) << 4), o[0], o[1], o[2], o[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            mbar_arrive_one(bar_vfull + 8 * (n & 1));
+        }
+    } else {
+        // ---------------- softmax, one row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+        const int row = tid;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        constexpr int kWide = QJL ? 256 : 128;
+        uint32_t n = 0;
+        while (flat < flat_end) {
+            const Segment g = next_segment();
+            const int node = g.t * a.positions + row / a.group;
+            const bool live = row < a.rows && node < a.nodes;
+            const uint64_t mask = live && a.mask ? a.mask[(int64_t)g.b * a.nodes + node] & (~0ull >> (64 - a.nodes)) : 0;
+            const int chain_end = a.mask ? -1 : live ? node + 1 : 0;
+            // ---- the queries (the products that read the ones before are done: their logits were here)
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.qop + (g.tile * a.rows + row) * kWide);
+#pragma unroll
+            for (int i = 0; i < kWide / 64; ++i) {
+                uint32_t r[32];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint4 x = row < a.rows ? src[8 * i + e] : make_uint4(0, 0, 0, 0);
+                    r[4 * e] = x.x, r[4 * e + 1] = x.y, r[4 * e + 2] = x.z, r[4 * e + 3] = x.w;
+                }
+                __syncwarp();
+                tmem_st32(t_q + lanes + 32 * i, r);
+            }
+            tmem_st_wait();
+            umma_fence_before();
+            mbar_arrive_one(bar_q);
+            float m_ref = -INFINITY;
+            uint64_t sum[2] = {0, 0};
+            for (int k = g.k; k < g.k_end; ++k, ++n) {
+                const uint32_t t_s = tmem + 128 * (n & 1) + lanes;
+                wait(bar_s + 8 * (n & 1), n >> 1 & 1);
+                __syncwarp();
+                umma_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s + 32 * i);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld_wait(s + 32 * i);
+                if ((k + 1) * kBlock > g.history) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t seen = seen_word(mask, chain_end, k * kBlock + 32 * x - g.history);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!(seen >> i & 1)) s[32 * x + i] = 0xff800000u;
+                    }
+                }
+                float top[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[i] = max3(__uint_as_float(s[i]), __uint_as_float(s[i + 4]), __uint_as_float(s[i + 8]));
+#pragma unroll
+                for (int i = 12; i < 124; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
+                float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                peak = fmaxf(peak, max3(__uint_as_float(s[124]), __uint_as_float(s[125]), fmaxf(__uint_as_float(s[126]), __uint_as_float(s[127]))));
+                if (k == g.k) {
+                    m_ref = peak;
+                } else {
+                    const bool raise = live && peak - m_ref > kLag;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        float keep = 1.f;
+                        if (raise) keep = exp2_hw(m_ref - peak), m_ref = peak;
+                        const uint64_t keep2 = f32x2(keep, keep);
+                        sum[0] = f32x2_mul(sum[0], keep2), sum[1] = f32x2_mul(sum[1], keep2);
+                        wait(bar_o, (n - 1) & 1);  // the values of the block before
+                        __syncwarp();
+                        umma_fence_after();
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t o[32];
+                            tmem_ld32(t_o + lanes + 32 * i, o);
+                            tmem_ld_wait(o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st32(t_o + lanes + 32 * i, o);
+                        }
+                    }
+                }
+                const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
+                const uint64_t shift2 = f32x2(shift, shift);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float x, y;
+                        f32x2_split(f32x2_add(f32x2(__uint_as_float(s[64 * half + 2 * i]), __uint_as_float(s[64 * half + 2 * i + 1])), shift2), x, y);
+                        x = exp2_hw(x), y = exp2_hw(y);
+                        sum[i & 1] = f32x2_add(sum[i & 1], f32x2(x, y));
+                        p[i] = pack16<false>(x, y);
+                    }
+                    tmem_st32(t_s + 32 * half, p);
+                }
+                tmem_st_wait();
+                umma_fence_before();
+                mbar_arrive_one(bar_p + 8 * (n & 1));
+            }
+            // ---- this piece of the tile's rows
+            float l0, l1;
+            f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
+            wait(bar_o, (n - 1) & 1);
+            __syncwarp();
+            umma_fence_after();
+            const int64_t r = (g.tile + blockIdx.x) * a.rows + row;
+            if (live) *reinterpret_cast<float2 *>(a.part_ml + 2 * r) = make_float2(m_ref, l0 + l1);
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                uint32_t o[32];
+                __syncwarp();
+                tmem_ld32(t_o + lanes + 32 * i, o);
+                tmem_ld_wait(o);
+                if (live)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(a.part_o + r * TQ_D + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            umma_fence_before();
+        }
+    }
+    if (lost) atomicExch(a.error_flag, 8);
+    umma_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        umma_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- join
+// kPrepRows rows a block: a warp merges the pieces of four of them, then a thread un-rotates one coordinate of all.
+template <typename T> __global__ void __launch_bounds__(128) tq_tree_join_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows) {
+    __shared__ float s_o[kPrepRows][TQ_D];
+    __shared__ int64_t s_to[kPrepRows];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
+    for (int i = warp; i < kPrepRows; i += 4) {
+        const int64_t r = (int64_t)blockIdx.x * kPrepRows + i, tile = r / a.rows;
+        const int in = (int)(r % a.rows), t = (int)(tile % a.tiles), h = (int)(tile / a.tiles % a.kv_heads), b = (int)(tile / a.tiles / a.kv_heads);
+        const int node = t * a.positions + in / a.group;
+        const bool live = r < n_rows && node < a.nodes;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live) {
+            const int history = entry_of(a, b).history;
+            int64_t first = a.prefix[b] + (int64_t)h * head_blocks(a, history);
+            for (int x = 0; x < t; ++x) first += tile_blocks(a, history, x);
+            const int64_t c0 = first / chunk, c1 = (first + tile_blocks(a, history, t) - 1) / chunk;
+            float m = -INFINITY, l = 0.f;
+            for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, a.part_ml[2 * ((tile + c) * a.rows + in)]);
+            for (int64_t c = c0; c <= c1; ++c) {
+                const int64_t p = (tile + c) * a.rows + in;
+                const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * p);
+                if (ml.y == 0.f) continue;  // (saw nothing there)
+                const float f = exp2f(ml.x - m);
+                const float4 v = reinterpret_cast<const float4 *>(a.part_o + p * TQ_D)[lane];
+                l += f * ml.y;
+                o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+            }
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+            o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+        *reinterpret_cast<float4 *>(&s_o[i][4 * lane]) = o;
+        if (lane == 0) s_to[i] = live ? b * a.ob + (h * a.group + in % a.group) * a.oh + node * a.ot : -1;
+    }
+    __syncthreads();
+    float acc[kPrepRows] = {};
+    for (int d = 0; d < TQ_D; d += 4) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __ldg(a.rot_v + (d + e) * TQ_D + threadIdx.x);
+#pragma unroll
+        for (int r = 0; r < kPrepRows; ++r) {
+            const float4 x = *reinterpret_cast<const float4 *>(&s_o[r][d]);
+            acc[r] += x.x * w[0] + x.y * w[1] + x.z * w[2] + x.w * w[3];
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kPrepRows; ++r)
+        if (s_to[r] >= 0) reinterpret_cast<T *>(a.out)[s_to[r] + threadIdx.x] = tq_from_float<T>(acc[r]);
 }
 
 bool aligned(const tq_dense_desc *d) {
     return !(((uintptr_t)d->data | (uintptr_t)(2 * (d->stride_b | d->stride_h | d->stride_t))) & 15);
 }
 
+struct Plan {
+    int positions, tiles, rows, ctas;
+    int64_t n_tiles;
+    size_t prefix, qop, ml, o, bytes;  // workspace offsets
+};
+Plan plan(const tq_ctx *ctx, int64_t batch, int q_heads, int kv_heads, int nodes, int tree_start) {
+    Plan p;
+    const int group = q_heads / kv_heads;
+    p.positions = kUmmaRows / group;
+    p.tiles = (nodes + p.positions - 1) / p.positions;
+    p.rows = (nodes < p.positions ? nodes : p.positions) * group;
+    p.n_tiles = batch * kv_heads * p.tiles;
+    const int64_t most = p.n_tiles * (((int64_t)tree_start + nodes + kBlock - 1) / kBlock);
+    p.ctas = most < ctx->sm_count ? (int)most : ctx->sm_count;
+    auto take = [at = (size_t)0](size_t bytes) mutable {
+        const size_t r = at;
+        at += (bytes + 255) / 256 * 256;
+        return r;
+    };
+    const size_t pieces = (size_t)(p.n_tiles + p.ctas) * p.rows;
+    p.prefix = take((batch + 1) * sizeof(int64_t));
+    p.qop = take((size_t)p.n_tiles * p.rows * (ctx->use_qjl ? 512 : 256));
+    p.ml = take(pieces * 2 * sizeof(float));
+    p.o = take(pieces * TQ_D * sizeof(float));
+    p.bytes = take(0);
+    return p;
+}
+
+template <int KB, int VB, bool QJL> cudaError_t launch_attend(const TreeArgs &a, int device, cudaStream_t stream) {
+    constexpr int smem = Layout<KB, VB, QJL>::kBytes;
+    const cudaError_t e = tq_allow_shared<tq_tree_kernel<KB, VB, QJL>>(device, smem);
+    if (e != cudaSuccess) return e;
+    tq_tree_kernel<KB, VB, QJL><<<a.ctas, kThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T> cudaError_t launch(const TreeArgs &a, int bits, bool qjl, int64_t n_rows, int device, cudaStream_t stream) {
+    const unsigned blocks = (unsigned)((n_rows + kPrepRows - 1) / kPrepRows);
+    if (qjl) tq_tree_prep_kernel<T, true><<<blocks, 256, 0, stream>>>(a, n_rows);
+    else tq_tree_prep_kernel<T, false><<<blocks, 128, 0, stream>>>(a, n_rows);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    switch (bits) {
+        case 2: e = qjl ? launch_attend<1, 2, true>(a, device, stream) : launch_attend<2, 2, false>(a, device, stream); break;
+        case 3: e = qjl ? launch_attend<2, 3, true>(a, device, stream) : launch_attend<3, 3, false>(a, device, stream); break;
+        case 4: e = qjl ? launch_attend<3, 4, true>(a, device, stream) : launch_attend<4, 4, false>(a, device, stream); break;
+        default: return cudaErrorInvalidValue;
+    }
+    if (e != cudaSuccess) return e;
+    tq_tree_join_kernel<T><<<blocks, 128, 0, stream>>>(a, n_rows);
+    return cudaGetLastError();
+}
+
 }  // namespace
 
-extern "C" size_t tq_tree_workspace_bytes(tq_ctx *ctx, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_nodes, int32_t n_tokens) {
-    return 0;
+extern "C" size_t tq_tree_workspace_bytes(tq_ctx *ctx, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_nodes, int32_t tree_start) {
+    if (!ctx || batch <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || q_heads / kv_heads > TQ_MAX_GROUPS || n_nodes <= 0 || tree_start < 0) return 0;
+    return plan(ctx, batch, q_heads, kv_heads, n_nodes, tree_start).bytes;
 }
 
 extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_heads, int32_t n_nodes, const tq_cache_desc *cache,
@@ -99,20 +620,26 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     if (n_nodes < 0 || tree_start < 0 || (int64_t)tree_start + n_nodes > cache->capacity) return TQ_ERR_ARG;
     if (q_heads <= 0 || q_heads % cache->kv_heads) return TQ_ERR_ARG;
     if (q_heads / cache->kv_heads > TQ_MAX_GROUPS || (tree_mask && n_nodes > TQ_MAX_TREE)) return TQ_ERR_UNSUPPORTED;
-    if (((uintptr_t)lengths & 3) || ((uintptr_t)tree_mask & 7)) return TQ_ERR_ARG;
+    if (((uintptr_t)lengths & 3) || ((uintptr_t)tree_mask & 7) || ((uintptr_t)workspace & 15)) return TQ_ERR_ARG;
     if (n_nodes == 0) return TQ_OK;
+    const Plan p = plan(ctx, cache->batch, q_heads, cache->kv_heads, n_nodes, tree_start);
+    const int64_t n_rows = p.n_tiles * p.rows;
+    if (n_rows / kPrepRows >= 0x7fffffff) return TQ_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < p.bytes) return TQ_ERR_WORKSPACE;
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
     TreeArgs a = {};
     a.k_codes = cache->k_codes, a.k_norms = cache->k_norms, a.k_signs = cache->k_signs, a.k_rnorms = cache->k_rnorms;
     a.v_codes = cache->v_codes, a.v_norms = cache->v_norms, a.cache_sb = cache->stride_b, a.cache_sh = cache->stride_h;
-    a.key_bits = ctx->key_bits, a.bits = ctx->bits, a.use_qjl = ctx->use_qjl, a.kv_heads = cache->kv_heads;
-    a.group = q_heads / cache->kv_heads, a.nodes = n_nodes, a.tree_start = tree_start;
+    a.batch = cache->batch, a.kv_heads = cache->kv_heads, a.group = q_heads / cache->kv_heads, a.nodes = n_nodes, a.tree_start = tree_start;
+    a.positions = p.positions, a.tiles = p.tiles, a.rows = p.rows, a.ctas = p.ctas;
     a.seq_start = cache->seq_start, a.lengths = lengths, a.mask = tree_mask;
     a.rot_k_t = ctx->rot_k_t, a.rot_v = ctx->rot_v, a.qjl_t = ctx->qjl_t, a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v;
     a.q = q->data, a.qb = q->stride_b, a.qh = q->stride_h, a.qt = q->stride_t;
     a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
-    const dim3 grid((n_nodes + 3) / 4, q_heads, cache->batch);
-    if (q->dtype == TQ_DTYPE_F16) tq_tree_kernel<__half><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    else tq_tree_kernel<__nv_bfloat16><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    TQ_CUDA_CHECK(cudaGetLastError());
+    a.prefix = reinterpret_cast<int64_t *>(ws + p.prefix), a.qop = reinterpret_cast<uint16_t *>(ws + p.qop);
+    a.part_ml = reinterpret_cast<float *>(ws + p.ml), a.part_o = reinterpret_cast<float *>(ws + p.o);
+    a.error_flag = ctx->error_flag;
+    TQ_CUDA_CHECK(q->dtype == TQ_DTYPE_F16 ? launch<__half>(a, ctx->bits, ctx->use_qjl != 0, n_rows, ctx->device, (cudaStream_t)stream)
+                                           : launch<__nv_bfloat16>(a, ctx->bits, ctx->use_qjl != 0, n_rows, ctx->device, (cudaStream_t)stream));
     return TQ_OK;
 }
