@@ -15,13 +15,15 @@
 // TMEM: S of two blocks, O, the queries, 128 columns each.
 #include <math.h>
 
+#include <type_traits>
+
 #include "tq_attn_tc.cuh"
+#include "tq_step_blocks.cuh"
 
 namespace {
 
 constexpr int kThreads = 512;
 constexpr int kBlock = 128;  // tokens of a block
-constexpr int kPrepRows = 16;
 
 struct TreeArgs {
     const uint8_t *k_codes, *k_signs, *v_codes;
@@ -31,7 +33,9 @@ struct TreeArgs {
     int positions, tiles, rows;  // nodes of a tile, tiles of a (batch entry, KV head), rows of a tile that hold something
     const int *seq_start, *lengths;
     const uint64_t *mask;
-    const float *rot_k_t, *rot_v, *qjl_t, *centers_k, *centers_v;
+    const uint16_t *image_k, *image_s, *image_v;  // R_k, S, R_v
+    float unscale_k, unscale_s, unscale_v;
+    const float *centers_k, *centers_v;
     const void *q;
     void *out;
     int64_t qb, qh, qt, ob, oh, ot;
@@ -61,62 +65,155 @@ __device__ __forceinline__ int head_blocks(const TreeArgs &a, int history) {
     return n;
 }
 
-// ---------------------------------------------------------------------------------------------------- queries
-// Operand rows [Rq | Sq], kPrepRows rows a block, a coordinate a thread.  Sketch coordinates lie in the order in which
-// the operand's signs do: (i, i + 16) side by side, see sign_pair.
-template <typename T, bool QJL> __global__ void __launch_bounds__(QJL ? 256 : 128) tq_tree_prep_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows) {
+// ---------------------------------------------------------------------------------------------------- 128 x 128 matrices
+// Rows times R_k^T, S^T or R_v, on the tensor core in two fp16 terms (see tq_umma.cuh).  A CTA takes up to 128 rows, so many that the
+// CTAs fill the SMs once; four threads to a row, 32 coordinates each.
+constexpr int kRowThreads = 512;
+
+struct RowPlace {
+    int b, h, head, node;  // head: of all query heads
+    int64_t tile;
+    int in;                // row of the tile
+    bool live;
+};
+__device__ __forceinline__ RowPlace place_of(const TreeArgs &a, int64_t r, int64_t n_rows) {
+    RowPlace p;
+    p.in = (int)(r % a.rows), p.tile = r / a.rows;
+    const int t = (int)(p.tile % a.tiles), g = p.in % a.group;
+    p.h = (int)(p.tile / a.tiles % a.kv_heads), p.b = (int)(p.tile / a.tiles / a.kv_heads);
+    p.head = p.h * a.group + g, p.node = t * a.positions + p.in / a.group;
+    p.live = r < n_rows && p.node < a.nodes;
+    return p;
+}
+
+// TMEM and the barriers of such a kernel, and its product: the rows are in TMEM as hi and lo terms at +256 and +320, the sums come at +128 i.
+struct RowTile {
+    uint32_t tmem, bar_image, bar_mma;
+    bool lost = false;
+    __device__ __forceinline__ void start(uint32_t *s_tmem, uint64_t *s_bars, uint32_t images, const uint16_t *image0, const uint16_t *image1) {
+        bar_image = smem_u32(s_bars), bar_mma = bar_image + 8;
+        if (threadIdx.x < 32) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)), "r"(512));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+        }
+        if (threadIdx.x == 32) {
+            mbar_init(bar_image, image1 ? 2 : 1), mbar_init(bar_mma, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            umma_load_image(images, image0, bar_image);
+            if (image1) umma_load_image(images + kUmmaImageBytes, image1, bar_image);
+        }
+        umma_fence_before();
+        __syncthreads();
+        umma_fence_after();
+        tmem = __shfl_sync(0xffffffffu, *s_tmem, 0);
+    }
+    // this thread's 32 coordinates of its row
+    __device__ __forceinline__ void put(const float (&x)[32], int part, uint32_t lanes) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) split_half2(f32x2(x[16 * c + 2 * i], x[16 * c + 2 * i + 1]), hi[i], lo[i]);
+            tmem_st8(tmem + 256 + lanes + 16 * part + 8 * c, hi), tmem_st8(tmem + 320 + lanes + 16 * part + 8 * c, lo);
+        }
+        tmem_st_wait();
+        umma_fence_before();
+        __syncthreads();
+    }
+    template <bool TRANSPOSED> __device__ __forceinline__ void multiply(uint32_t images, int n) {
+        if (threadIdx.x < 32 && elect_one()) {
+            umma_fence_after();
+            if (!mbar_wait(bar_image, 0)) lost = true;
+            for (int i = 0; i < n; ++i) umma_issue<2, TRANSPOSED>(tmem + 128 * i, tmem + 256, tmem + 320, images + i * kUmmaImageBytes);
+            umma_commit(bar_mma);
+        }
+        __syncwarp();
+        if (!mbar_wait(bar_mma, 0)) lost = true;
+        __syncwarp();
+        umma_fence_after();
+    }
+    __device__ __forceinline__ void finish(int *error_flag) {
+        if (lost) atomicExch(error_flag, 8);
+        umma_fence_before();
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            umma_fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
+        }
+    }
+};
+
+// Operand rows [Rq | Sq].  Sketch coordinates lie in the order in which the operand's signs do, (i, i + 16) of 32 side by side.
+template <typename T, bool QJL> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_prep_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows, int per_cta) {
     constexpr int kWide = QJL ? 256 : 128;
-    __shared__ float s_q[kPrepRows][TQ_D];
-    if (blockIdx.x == 0 && threadIdx.x < 32) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_bars[2];
+    __shared__ uint32_t s_tmem;
+    const uint32_t images = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    tq_launch_dependents();
+    RowTile tile;
+    tile.start(&s_tmem, s_bars, images, a.image_k, QJL ? a.image_s : nullptr);
+    if (blockIdx.x == 0 && threadIdx.x >= kRowThreads - 32) {  // (rows of the last warp are few, or there are many other blocks)
+        const int lane = threadIdx.x & 31;
         int64_t before = 0;
         for (int b0 = 0; b0 < a.batch; b0 += 32) {
-            const int b = b0 + threadIdx.x;
+            const int b = b0 + lane;
             int64_t n = b < a.batch ? (int64_t)head_blocks(a, entry_of(a, b).history) * a.kv_heads : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t x = __shfl_up_sync(0xffffffffu, n, o);
-                if (threadIdx.x >= o) n += x;
+                if (lane >= o) n += x;
             }
             if (b < a.batch) a.prefix[b + 1] = before + n;
             before += __shfl_sync(0xffffffffu, n, 31);
         }
-        if (threadIdx.x == 0) a.prefix[0] = 0;
+        if (lane == 0) a.prefix[0] = 0;
     }
-    const int64_t row0 = (int64_t)blockIdx.x * kPrepRows;
-    const float scale = 0.08838834764831845f * 1.4426950408889634f;
-    for (int i = threadIdx.x; i < kPrepRows * TQ_D; i += kWide) {
-        const int64_t r = row0 + i / TQ_D;
-        float x = 0.f;
-        if (r < n_rows) {
-            const int in = (int)(r % a.rows);
-            const int64_t tile = r / a.rows;
-            const int t = (int)(tile % a.tiles), h = (int)(tile / a.tiles % a.kv_heads), b = (int)(tile / a.tiles / a.kv_heads);
-            const int node = t * a.positions + in / a.group;
-            if (node < a.nodes)
-                x = tq_to_float<T>(reinterpret_cast<const T *>(a.q)[b * a.qb + (h * a.group + in % a.group) * a.qh + node * a.qt + i % TQ_D]) * scale;
-        }
-        s_q[i / TQ_D][i % TQ_D] = x;
-    }
-    __syncthreads();
-    const int c = threadIdx.x & 127;
-    const bool sketch = threadIdx.x >= 128;
-    const int from = sketch ? (c & ~31) + (c & 1) * 16 + ((c & 31) >> 1) : c;  // the coordinate at place c
-    const float *m = (sketch ? a.qjl_t : a.rot_k_t) + from;
-    float acc[kPrepRows] = {};
-    for (int d = 0; d < TQ_D; d += 4) {
-        float w[4];
+    const int row = threadIdx.x & 127, part = threadIdx.x >> 7;
+    const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
+    const int64_t r = (int64_t)blockIdx.x * per_cta + row;
+    const bool mine = row < per_cta && r < n_rows;
+    float x[32] = {};
+    if (mine) {
+        const RowPlace p = place_of(a, r, n_rows);
+        if (p.live) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + p.b * a.qb + p.head * a.qh + p.node * a.qt) + 4 * part;
+            const float scale = 0.08838834764831845f * 1.4426950408889634f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = __ldg(m + (d + e) * TQ_D);
+            for (int i = 0; i < 4; ++i) {
+                const uint4 v = __ldg(src + i);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int r = 0; r < kPrepRows; ++r) {
-            const float4 x = *reinterpret_cast<const float4 *>(&s_q[r][d]);
-            acc[r] += x.x * w[0] + x.y * w[1] + x.z * w[2] + x.w * w[3];
+                for (int e = 0; e < 4; ++e) {
+                    const T *pair = reinterpret_cast<const T *>(&w[e]);
+                    x[8 * i + 2 * e] = tq_to_float<T>(pair[0]) * scale, x[8 * i + 2 * e + 1] = tq_to_float<T>(pair[1]) * scale;
+                }
+            }
         }
     }
-    const float f = sketch ? 1.2533141373155003f / (float)TQ_D : 1.f;
+    __syncwarp();
+    tile.put(x, part, lanes);
+    tile.multiply<false>(images, QJL ? 2 : 1);
 #pragma unroll
-    for (int r = 0; r < kPrepRows; ++r)
-        if (row0 + r < n_rows) a.qop[(row0 + r) * kWide + threadIdx.x] = tq_float_to_half_bits(acc[r] * f);
+    for (int i = 0; i < (QJL ? 2 : 1); ++i) {
+        const float f = i ? a.unscale_s * (1.2533141373155003f / (float)TQ_D) : a.unscale_k;
+        uint32_t y[32], o[16];
+        __syncwarp();
+        tmem_ld32(tile.tmem + 128 * i + lanes + 32 * part, y);
+        tmem_ld_wait(y);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int lo = i ? e : 2 * e, hi = i ? e + 16 : 2 * e + 1;
+            o[e] = half2_bits(__uint_as_float(y[lo]) * f, __uint_as_float(y[hi]) * f);
+        }
+        if (mine) {
+            uint4 *dst = reinterpret_cast<uint4 *>(a.qop + r * kWide + 128 * i + 32 * part);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+    }
+    tile.finish(a.error_flag);
 }
 
 // ---------------------------------------------------------------------------------------------------- attention
@@ -180,19 +277,23 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     {
-        auto fill = [&](uint32_t table, int bytes, int slot, int bits, const float *centers) {
+        const float ck = a.centers_k[lane & 15], cv = a.centers_v[lane & 15];
+        auto fill = [&](uint32_t table, int slot, int bits, float centre) {
             const int copies = slot / 4;
-            for (int i = tid; i < bytes / 4; i += kThreads) {
+            for (int i = tid; i < (copies << 2 * bits); i += kThreads) {  // (whole warps)
                 const int e = i / copies;
-                asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(table + 4 * i), "r"(half2_bits(centers[e & ((1 << bits) - 1)], centers[e >> bits])) : "memory");
+                const float lo = __shfl_sync(0xffffffffu, centre, e & ((1 << bits) - 1)), hi = __shfl_sync(0xffffffffu, centre, e >> bits);
+                asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(table + 4 * i), "r"(half2_bits(lo, hi)) : "memory");
             }
         };
-        fill(table_k, L::kKeyTable, L::kKeySlot, KB, a.centers_k);
-        fill(table_v, L::kValueTable, L::kValueSlot, VB, a.centers_v);
+        fill(table_k, L::kKeySlot, KB, ck);
+        fill(table_v, L::kValueSlot, VB, cv);
     }
     umma_fence_before();
     __syncthreads();
     umma_fence_after();
+    tq_grid_dependency_wait();
+    tq_launch_dependents();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), t_o = tmem + 256, t_q = tmem + 384;
 
     // ---- this CTA's blocks: [flat, flat_end) of all tiles' blocks laid end to end
@@ -203,15 +304,13 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         int b, h, t, history, start, k, k_end;
         int64_t tile;
     };
-    int b_at = 0;
-    if (flat < flat_end) {
-        int hi = a.batch;  // the entry that holds block `flat`
-        while (hi - b_at > 1) {
-            const int mid = (b_at + hi) >> 1;
-            if (a.prefix[mid] <= flat) b_at = mid;
-            else hi = mid;
+    int b_at = 0;  // the entry that holds block `flat`
+    if (flat < flat_end)
+        for (int b0 = 0, n = 32; n == 32; b0 += 32) {
+            const int64_t end = a.prefix[min(b0 + lane + 1, a.batch)];
+            n = __popc(__ballot_sync(0xffffffffu, b0 + lane < a.batch && end <= flat));
+            b_at += n;
         }
-    }
     int64_t b_first = flat < flat_end ? a.prefix[b_at] : 0, b_next = flat < flat_end ? a.prefix[b_at + 1] : 0;
     auto next_segment = [&]() {
         while (flat >= b_next) ++b_at, b_first = b_next, b_next = a.prefix[b_at + 1];
@@ -493,55 +592,77 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
 }
 
 // ---------------------------------------------------------------------------------------------------- join
-// kPrepRows rows a block: a warp merges the pieces of four of them, then a thread un-rotates one coordinate of all.
-template <typename T> __global__ void __launch_bounds__(128) tq_tree_join_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows) {
-    __shared__ float s_o[kPrepRows][TQ_D];
-    __shared__ int64_t s_to[kPrepRows];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
-    for (int i = warp; i < kPrepRows; i += 4) {
-        const int64_t r = (int64_t)blockIdx.x * kPrepRows + i, tile = r / a.rows;
-        const int in = (int)(r % a.rows), t = (int)(tile % a.tiles), h = (int)(tile / a.tiles % a.kv_heads), b = (int)(tile / a.tiles / a.kv_heads);
-        const int node = t * a.positions + in / a.group;
-        const bool live = r < n_rows && node < a.nodes;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (live) {
-            const int history = entry_of(a, b).history;
-            int64_t first = a.prefix[b] + (int64_t)h * head_blocks(a, history);
-            for (int x = 0; x < t; ++x) first += tile_blocks(a, history, x);
-            const int64_t c0 = first / chunk, c1 = (first + tile_blocks(a, history, t) - 1) / chunk;
-            float m = -INFINITY, l = 0.f;
-            for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, a.part_ml[2 * ((tile + c) * a.rows + in)]);
-            for (int64_t c = c0; c <= c1; ++c) {
-                const int64_t p = (tile + c) * a.rows + in;
-                const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * p);
-                if (ml.y == 0.f) continue;  // (saw nothing there)
-                const float f = exp2f(ml.x - m);
-                const float4 v = reinterpret_cast<const float4 *>(a.part_o + p * TQ_D)[lane];
-                l += f * ml.y;
-                o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+// Merges a row's pieces, brings its largest coordinate to [2^13, 2^14) for the fp16 terms, un-rotates and rounds.
+template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_join_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows, int per_cta) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_bars[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ float s_most[4][128];
+    const uint32_t images = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    RowTile tile;
+    tile.start(&s_tmem, s_bars, images, a.image_v, nullptr);
+    const int row = threadIdx.x & 127, part = threadIdx.x >> 7;
+    const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
+    const int64_t r = (int64_t)blockIdx.x * per_cta + row;
+    RowPlace p = {};
+    if (row < per_cta && r < n_rows) p = place_of(a, r, n_rows);
+    tq_grid_dependency_wait();
+    float o[32] = {};
+    if (p.live) {
+        const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
+        const int history = entry_of(a, p.b).history, t = (int)(p.tile % a.tiles);
+        int64_t first = a.prefix[p.b] + (int64_t)p.h * head_blocks(a, history);
+        for (int x = 0; x < t; ++x) first += tile_blocks(a, history, x);
+        const int64_t c0 = first / chunk, c1 = (first + tile_blocks(a, history, t) - 1) / chunk;
+        float m = -INFINITY, l = 0.f;
+        for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, a.part_ml[2 * ((p.tile + c) * a.rows + p.in)]);
+        for (int64_t c = c0; c <= c1; ++c) {
+            const int64_t piece = (p.tile + c) * a.rows + p.in;
+            const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * piece);
+            const float4 *src = reinterpret_cast<const float4 *>(a.part_o + piece * TQ_D + 32 * part);
+            const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - m);  // (a piece in which the row saw nothing)
+            l += f * ml.y;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 v = src[i];
+                o[4 * i] += f * v.x, o[4 * i + 1] += f * v.y, o[4 * i + 2] += f * v.z, o[4 * i + 3] += f * v.w;
             }
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-            o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         }
-        *reinterpret_cast<float4 *>(&s_o[i][4 * lane]) = o;
-        if (lane == 0) s_to[i] = live ? b * a.ob + (h * a.group + in % a.group) * a.oh + node * a.ot : -1;
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] *= inv;
     }
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(o[i]));
+    s_most[part][row] = most;
     __syncthreads();
-    float acc[kPrepRows] = {};
-    for (int d = 0; d < TQ_D; d += 4) {
-        float w[4];
+    most = fmaxf(fmaxf(s_most[0][row], s_most[1][row]), fmaxf(s_most[2][row], s_most[3][row]));
+    // the power of two from the exponent's bits; what is too small for one is left as it is, and so is infinity
+    const int exponent = (int)(__float_as_uint(most) >> 23);
+    const int up = exponent == 0 || exponent == 255 ? 0 : min(13 + 127 - exponent, 120);
+    const float raise = __uint_as_float((uint32_t)(127 + up) << 23), lower = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = __ldg(a.rot_v + (d + e) * TQ_D + threadIdx.x);
+    for (int i = 0; i < 32; ++i) o[i] *= raise;
+    __syncwarp();
+    tile.put(o, part, lanes);
+    tile.multiply<true>(images, 1);
+    uint32_t y[32];
+    tmem_ld32(tile.tmem + lanes + 32 * part, y);
+    tmem_ld_wait(y);
+    if (p.live) {
+        const float f = a.unscale_v * lower;
+        uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + p.b * a.ob + p.head * a.oh + p.node * a.ot + 32 * part);
 #pragma unroll
-        for (int r = 0; r < kPrepRows; ++r) {
-            const float4 x = *reinterpret_cast<const float4 *>(&s_o[r][d]);
-            acc[r] += x.x * w[0] + x.y * w[1] + x.z * w[2] + x.w * w[3];
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = pack16<std::is_same<T, __nv_bfloat16>::value>(__uint_as_float(y[8 * i + 2 * e]) * f, __uint_as_float(y[8 * i + 2 * e + 1]) * f);
+            dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-#pragma unroll
-    for (int r = 0; r < kPrepRows; ++r)
-        if (s_to[r] >= 0) reinterpret_cast<T *>(a.out)[s_to[r] + threadIdx.x] = tq_from_float<T>(acc[r]);
+    tile.finish(a.error_flag);
 }
 
 bool aligned(const tq_dense_desc *d) {
@@ -579,26 +700,33 @@ Plan plan(const tq_ctx *ctx, int64_t batch, int q_heads, int kv_heads, int nodes
 template <int KB, int VB, bool QJL> cudaError_t launch_attend(const TreeArgs &a, int device, cudaStream_t stream) {
     constexpr int smem = Layout<KB, VB, QJL>::kBytes;
     const cudaError_t e = tq_allow_shared<tq_tree_kernel<KB, VB, QJL>>(device, smem);
-    if (e != cudaSuccess) return e;
-    tq_tree_kernel<KB, VB, QJL><<<a.ctas, kThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+    return e != cudaSuccess ? e : tq_launch_kernel(tq_tree_kernel<KB, VB, QJL>, dim3(a.ctas), dim3(kThreads), smem, stream, true, a);
 }
 
-template <typename T> cudaError_t launch(const TreeArgs &a, int bits, bool qjl, int64_t n_rows, int device, cudaStream_t stream) {
-    const unsigned blocks = (unsigned)((n_rows + kPrepRows - 1) / kPrepRows);
-    if (qjl) tq_tree_prep_kernel<T, true><<<blocks, 256, 0, stream>>>(a, n_rows);
-    else tq_tree_prep_kernel<T, false><<<blocks, 128, 0, stream>>>(a, n_rows);
-    cudaError_t e = cudaGetLastError();
+template <typename T, bool QJL> cudaError_t launch_prep(const TreeArgs &a, int64_t n_rows, unsigned blocks, int per_cta, int device, cudaStream_t stream) {
+    constexpr int smem = (QJL ? 2 : 1) * kUmmaImageBytes + 1024;
+    const cudaError_t e = tq_allow_shared<tq_tree_prep_kernel<T, QJL>>(device, smem);
+    return e != cudaSuccess ? e : tq_launch_kernel(tq_tree_prep_kernel<T, QJL>, dim3(blocks), dim3(kRowThreads), smem, stream, false, a, n_rows, per_cta);
+}
+
+template <typename T> cudaError_t launch(const TreeArgs &a, const tq_ctx *ctx, int64_t n_rows, cudaStream_t stream) {
+    const bool qjl = ctx->use_qjl != 0;
+    const int device = ctx->device;
+    const int64_t share = ((n_rows + ctx->sm_count - 1) / ctx->sm_count + 7) / 8 * 8;
+    const int per_cta = share < kUmmaRows ? (int)share : kUmmaRows;
+    const unsigned blocks = (unsigned)((n_rows + per_cta - 1) / per_cta);
+    cudaError_t e = qjl ? launch_prep<T, true>(a, n_rows, blocks, per_cta, device, stream) : launch_prep<T, false>(a, n_rows, blocks, per_cta, device, stream);
     if (e != cudaSuccess) return e;
-    switch (bits) {
+    switch (ctx->bits) {
         case 2: e = qjl ? launch_attend<1, 2, true>(a, device, stream) : launch_attend<2, 2, false>(a, device, stream); break;
         case 3: e = qjl ? launch_attend<2, 3, true>(a, device, stream) : launch_attend<3, 3, false>(a, device, stream); break;
         case 4: e = qjl ? launch_attend<3, 4, true>(a, device, stream) : launch_attend<4, 4, false>(a, device, stream); break;
         default: return cudaErrorInvalidValue;
     }
     if (e != cudaSuccess) return e;
-    tq_tree_join_kernel<T><<<blocks, 128, 0, stream>>>(a, n_rows);
-    return cudaGetLastError();
+    constexpr int smem = kUmmaImageBytes + 1024;
+    e = tq_allow_shared<tq_tree_join_kernel<T>>(device, smem);
+    return e != cudaSuccess ? e : tq_launch_kernel(tq_tree_join_kernel<T>, dim3(blocks), dim3(kRowThreads), smem, stream, true, a, n_rows, per_cta);
 }
 
 }  // namespace
@@ -624,7 +752,7 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     if (n_nodes == 0) return TQ_OK;
     const Plan p = plan(ctx, cache->batch, q_heads, cache->kv_heads, n_nodes, tree_start);
     const int64_t n_rows = p.n_tiles * p.rows;
-    if (n_rows / kPrepRows >= 0x7fffffff) return TQ_ERR_UNSUPPORTED;
+    if (n_rows / 8 >= 0x7fffffff) return TQ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < p.bytes) return TQ_ERR_WORKSPACE;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     TreeArgs a = {};
@@ -633,13 +761,15 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     a.batch = cache->batch, a.kv_heads = cache->kv_heads, a.group = q_heads / cache->kv_heads, a.nodes = n_nodes, a.tree_start = tree_start;
     a.positions = p.positions, a.tiles = p.tiles, a.rows = p.rows, a.ctas = p.ctas;
     a.seq_start = cache->seq_start, a.lengths = lengths, a.mask = tree_mask;
-    a.rot_k_t = ctx->rot_k_t, a.rot_v = ctx->rot_v, a.qjl_t = ctx->qjl_t, a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v;
+    a.image_k = ctx->img_rot_k.data, a.image_s = ctx->img_qjl.data, a.image_v = ctx->img_rot_v.data;
+    a.unscale_k = kUmmaRestore * ctx->img_rot_k.unscale, a.unscale_s = kUmmaRestore * ctx->img_qjl.unscale, a.unscale_v = kUmmaRestore * ctx->img_rot_v.unscale;
+    a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v;
     a.q = q->data, a.qb = q->stride_b, a.qh = q->stride_h, a.qt = q->stride_t;
     a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
     a.prefix = reinterpret_cast<int64_t *>(ws + p.prefix), a.qop = reinterpret_cast<uint16_t *>(ws + p.qop);
     a.part_ml = reinterpret_cast<float *>(ws + p.ml), a.part_o = reinterpret_cast<float *>(ws + p.o);
     a.error_flag = ctx->error_flag;
-    TQ_CUDA_CHECK(q->dtype == TQ_DTYPE_F16 ? launch<__half>(a, ctx->bits, ctx->use_qjl != 0, n_rows, ctx->device, (cudaStream_t)stream)
-                                           : launch<__nv_bfloat16>(a, ctx->bits, ctx->use_qjl != 0, n_rows, ctx->device, (cudaStream_t)stream));
+    TQ_CUDA_CHECK(q->dtype == TQ_DTYPE_F16 ? launch<__half>(a, ctx, n_rows, (cudaStream_t)stream)
+                                           : launch<__nv_bfloat16>(a, ctx, n_rows, (cudaStream_t)stream));
     return TQ_OK;
 }
