@@ -615,13 +615,17 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
         for (int x = 0; x < t; ++x) first += tile_blocks(a, history, x);
         const int64_t c0 = first / chunk, c1 = (first + tile_blocks(a, history, t) - 1) / chunk;
         float m = -INFINITY, l = 0.f;
-        for (int64_t c = c0; c <= c1; ++c) m = fmaxf(m, a.part_ml[2 * ((p.tile + c) * a.rows + p.in)]);
-        for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t piece = (p.tile + c) * a.rows + p.in;
-            const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * piece);
-            const float4 *src = reinterpret_cast<const float4 *>(a.part_o + piece * TQ_D + 32 * part);
-            const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - m);  // (a piece in which the row saw nothing)
-            l += f * ml.y;
+        const int64_t piece0 = (p.tile + c0) * a.rows + p.in;
+        const int n = (int)(c1 - c0) + 1;
+        const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + piece0;
+#pragma unroll 8
+        for (int c = 0; c < n; ++c) m = fmaxf(m, ml[(int64_t)c * a.rows].x);
+#pragma unroll 2
+        for (int c = 0; c < n; ++c) {
+            const float2 x = ml[(int64_t)c * a.rows];
+            const float4 *src = reinterpret_cast<const float4 *>(a.part_o + (piece0 + (int64_t)c * a.rows) * TQ_D + 32 * part);
+            const float f = x.y == 0.f ? 0.f : exp2f(x.x - m);  // (a piece in which the row saw nothing)
+            l += f * x.y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float4 v = src[i];

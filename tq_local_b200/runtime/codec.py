@@ -42,23 +42,32 @@ def dense_desc(t: torch.Tensor) -> ffi.DenseDesc:
     return ffi.DenseDesc(t.data_ptr(), tq_dtype(t.dtype), t.stride(0), t.stride(1), t.stride(2))
 
 
-def aligned_view(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself when kernels that move 16 bytes at a time can address it (contiguous last axis, rows on 16-byte
-    boundaries, no axis repeated by a stride of 0), else a contiguous copy."""
+def _addressable(t: torch.Tensor) -> bool:
+    """Whether kernels that move 16 bytes at a time can address the rows of ``t``: contiguous last axis, rows on 16-byte
+    boundaries, no axis repeated by a stride of 0 (an axis of one element has no stride of its own)."""
+    *outer, last = t.stride()
+    if last != 1 or t.data_ptr() & 15:
+        return False
     step = 16 // t.element_size()
-    fits = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s > 0 and s % step == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-    return t if fits else t.clone(memory_format=torch.contiguous_format)
+    for n, s in zip(t.shape, outer):
+        if n > 1 and (s == 0 or s % step):
+            return False
+    return True
+
+
+def aligned_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when kernels can address it (``_addressable``), else a contiguous copy."""
+    return t if _addressable(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def strided_desc(t: torch.Tensor) -> ffi.DenseDesc:
-    """``dense_desc`` of an ``aligned_view``: an axis of one element has no stride of its own."""
-    strides = [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
-    return ffi.DenseDesc(t.data_ptr(), tq_dtype(t.dtype), *strides)
+    """``dense_desc`` of an ``aligned_view`` [B, H, T, 128]."""
+    (b, h, n, _), (sb, sh, st, _) = t.shape, t.stride()
+    return ffi.DenseDesc(t.data_ptr(), _TORCH_TO_TQ[t.dtype], sb if b > 1 else 0, sh if h > 1 else 0, st if n > 1 else 0)
 
 
 def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
         raise ffi.TQError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 

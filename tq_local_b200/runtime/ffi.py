@@ -180,6 +180,21 @@ def lib() -> C.CDLL:
     return L
 
 
+def launch(name: str, device, args: tuple) -> None:
+    """Library call ``name(*args, stream)`` on the current stream of ``device`` (a CUDA device with an index), checked.  A device
+    that is current already is left alone: entering it costs as much as the call's other host work."""
+    import torch
+
+    fn, index = getattr(_lib or lib(), name), device.index
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status, name)
+
+
 def check(status: int, what: str) -> None:
     if status == 0:
         return

@@ -413,7 +413,7 @@ class PackedStore:
 
     # ------------------------------------------------------------------ drafted tokens
     def _int32(self, t: torch.Tensor, shape: tuple, what: str) -> torch.Tensor:
-        if t.dtype != torch.int32 or t.device != self.codec.device or tuple(t.shape) != shape:
+        if t.dtype != torch.int32 or t.device != self.codec.device or t.shape != shape:
             raise ValueError(f"{what} must be an int32 tensor {list(shape)} on {self.codec.device}")
         return t.contiguous()
 
@@ -448,11 +448,11 @@ class PackedStore:
             return out
         q = aligned_view(q)
         need = int(ffi.lib().tq_tree_workspace_bytes(self.codec.handle, b, hq, self.kv_heads, t, start))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # (the call's own: calls may overlap or be recorded)
         qd, od = strided_desc(q), strided_desc(out)
-        self._call("tq_tree_attn", self.codec.handle, C.byref(qd), hq, t, self._desc_ref, start,
-                   None if lengths is None else lengths.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(),
-                   None if ws is None else ws.data_ptr(), need, C.byref(od))
+        ffi.launch("tq_tree_attn", self.codec.device, (
+            self.codec.handle, C.byref(qd), hq, t, self._desc_ref, start, None if lengths is None else lengths.data_ptr(),
+            None if tree_mask is None else tree_mask.data_ptr(), ws.data_ptr(), need, C.byref(od)))
         return out
 
     def keep_tokens(self, path: torch.Tensor, counts: torch.Tensor, *, tree_start: int, lengths: torch.Tensor) -> torch.Tensor:
@@ -470,8 +470,9 @@ class PackedStore:
         if path.shape[1] == 0:
             return lengths.clone()
         out = torch.empty_like(lengths)
-        self._call("tq_cache_keep_tokens", self.codec.handle, self._desc_ref, int(tree_start), path.data_ptr(), int(path.shape[1]),
-                   counts.data_ptr(), lengths.data_ptr(), out.data_ptr())
+        ffi.launch("tq_cache_keep_tokens", self.codec.device, (
+            self.codec.handle, self._desc_ref, int(tree_start), path.data_ptr(), int(path.shape[1]), counts.data_ptr(),
+            lengths.data_ptr(), out.data_ptr()))
         return out
 
     def truncate(self, length: int) -> None:
@@ -495,8 +496,8 @@ class PackedStore:
         if index.numel() != self.batch or not 0 <= int(lo) <= hi <= self.length:
             raise ValueError(f"select_rows takes {self.batch} rows and tokens within [0, {self.length}), got {index.numel()} and [{lo}, {hi})")
         starts = None if self._seq_start is None else torch.empty_like(self._seq_start)
-        self._call("tq_cache_select_rows", self.codec.handle, self._desc_ref, self._desc_ref, index.data_ptr(), int(lo), hi,
-                   None if starts is None else starts.data_ptr())
+        ffi.launch("tq_cache_select_rows", self.codec.device, (
+            self.codec.handle, self._desc_ref, self._desc_ref, index.data_ptr(), int(lo), hi, None if starts is None else starts.data_ptr()))
         if starts is not None:
             self.set_seq_start(starts)
 
@@ -510,8 +511,8 @@ class PackedStore:
         starts = None
         if self._seq_start is not None:
             starts = torch.empty(other.batch, dtype=torch.int32, device=self.codec.device)
-        self._call("tq_cache_select_rows", self.codec.handle, self._desc_ref, other._desc_ref, index.data_ptr(), 0, self.length,
-                   None if starts is None else starts.data_ptr())
+        ffi.launch("tq_cache_select_rows", self.codec.device, (
+            self.codec.handle, self._desc_ref, other._desc_ref, index.data_ptr(), 0, self.length, None if starts is None else starts.data_ptr()))
         other.length = self.length
         other.set_seq_start(starts)
         return other

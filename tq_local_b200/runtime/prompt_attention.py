@@ -15,24 +15,29 @@ from tq_local_b200.runtime import ffi
 from tq_local_b200.runtime.codec import aligned_view, refuse_grad, strided_desc
 
 
-def _check(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, dims: int, heads_axis: int) -> None:
-    shapes = f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}"
-    if query.dim() != dims or key.dim() != dims or key.shape != value.shape or query.shape[-1] != 128 or key.shape[-1] != 128:
-        raise ValueError(f"expected queries, keys and values of {dims} axes with 128 coordinates, keys and values alike; got {shapes}")
-    hq, hkv = int(query.shape[heads_axis]), int(key.shape[heads_axis])
-    if hkv == 0 or hq == 0 or hq % hkv:
-        raise ValueError(f"query heads must be a multiple of KV heads, got {shapes}")
-    if query.device.type != "cuda":
+_SCALE = 128 ** -0.5
+
+
+def _check(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, dims: int) -> None:
+    """Shapes, devices and types of [..., heads, ..., 128] tensors whose heads are the second axis."""
+    qs, ks = query.shape, key.shape
+    if len(qs) != dims or len(ks) != dims or ks != value.shape or qs[-1] != 128 or ks[-1] != 128:
+        raise ValueError(f"expected queries, keys and values of {dims} axes with 128 coordinates, keys and values alike; got {tuple(qs)}, "
+                         f"{tuple(ks)}, {tuple(value.shape)}")
+    if ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
+        raise ValueError(f"query heads must be a multiple of KV heads, got {tuple(qs)}, {tuple(ks)}")
+    device, dtype = query.device, query.dtype
+    if device.type != "cuda":
         raise ffi.TQError("TurboQuant-B200 runs on CUDA devices only; there is no CPU path")
-    if key.device != query.device or value.device != query.device:
-        raise ffi.TQError(f"queries on {query.device}, keys on {key.device}, values on {value.device}")
-    if query.dtype not in (torch.float16, torch.bfloat16) or key.dtype != query.dtype or value.dtype != query.dtype:
-        raise TypeError(f"expected float16 or bfloat16 for all three, got {query.dtype}, {key.dtype}, {value.dtype}")
+    if key.device != device or value.device != device:
+        raise ffi.TQError(f"queries on {device}, keys on {key.device}, values on {value.device}")
+    if dtype not in (torch.float16, torch.bfloat16) or key.dtype != dtype or value.dtype != dtype:
+        raise TypeError(f"expected float16 or bfloat16 for all three, got {dtype}, {key.dtype}, {value.dtype}")
     refuse_grad("prompt attention", query, key, value)
 
 
 def _int32(t: torch.Tensor, shape: tuple, device: torch.device, what: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+    if t.dtype != torch.int32 or t.device != device or t.shape != shape:
         raise ValueError(f"{what} must be an int32 tensor {list(shape)} on {device}")
     return t.contiguous()
 
@@ -45,18 +50,10 @@ def _output(out: torch.Tensor | None, query: torch.Tensor, make) -> torch.Tensor
     return out
 
 
-def _launch(name: str, device: torch.device, workspace_args: tuple, *args_of_workspace_and_stream) -> None:
-    before, after = args_of_workspace_and_stream
-    lib = ffi.lib()
-    need = int(lib.tq_prompt_workspace_bytes(*workspace_args))
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    args = (*before, None if ws is None else ws.data_ptr(), need, *after, torch.cuda.current_stream(device).cuda_stream)
-    if torch.cuda.current_device() == device.index:
-        status = getattr(lib, name)(*args)
-    else:
-        with torch.cuda.device(device):
-            status = getattr(lib, name)(*args)
-    ffi.check(status, name)
+def _workspace(device: torch.device, *shape: int) -> tuple[torch.Tensor | None, int]:
+    """Scratch of this call alone (calls may overlap or be recorded); mostly none is needed."""
+    need = ffi.lib().tq_prompt_workspace_bytes(*shape)
+    return (torch.empty(need, dtype=torch.uint8, device=device) if need else None), need
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: float | None = None,
@@ -65,10 +62,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     [B, Sq, Hq, 128].  Causal: query ``i`` sees the keys up to ``i + Skv - Sq`` (so ``Sq`` < ``Skv`` is a chunk behind
     ``Skv - Sq`` earlier tokens).  ``seq_start`` (int32 [B] on the device): entry ``b`` attends keys from there on, a
     left-padded batch; a query that sees no key gets zeros.  ``scale`` defaults to 1/sqrt(128)."""
-    _check(query, key, value, 4, 1)
-    b, hq, n_q = int(query.shape[0]), int(query.shape[1]), int(query.shape[2])
-    hkv, n_kv = int(key.shape[1]), int(key.shape[2])
-    if key.shape[0] != b or (causal and n_kv < n_q):
+    _check(query, key, value, 4)
+    (b, hq, n_q, _), (b_kv, hkv, n_kv, _) = query.shape, key.shape
+    if b_kv != b or (causal and n_kv < n_q):
         raise ValueError(f"keys {tuple(key.shape)} do not go with queries {tuple(query.shape)}" + (" under a causal mask" if causal else ""))
     if seq_start is not None:
         seq_start = _int32(seq_start, (b,), query.device, "seq_start")
@@ -79,9 +75,10 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         return out.zero_()
     q, k, v = aligned_view(query), aligned_view(key), aligned_view(value)
     qd, kd, vd, od = strided_desc(q), strided_desc(k), strided_desc(v), strided_desc(out)
-    _launch("tq_prompt_attn", query.device, (b, hq, hkv, n_q, n_kv),
-            (C.byref(qd), C.byref(kd), C.byref(vd), b, hq, hkv, n_q, n_kv, None if seq_start is None else seq_start.data_ptr(),
-             128 ** -0.5 if scale is None else float(scale), int(causal)), (C.byref(od),))
+    ws, need = _workspace(query.device, b, hq, hkv, n_q, n_kv)
+    ffi.launch("tq_prompt_attn", query.device, (
+        C.byref(qd), C.byref(kd), C.byref(vd), b, hq, hkv, n_q, n_kv, None if seq_start is None else seq_start.data_ptr(),
+        _SCALE if scale is None else float(scale), int(causal), None if ws is None else ws.data_ptr(), need, C.byref(od)))
     return out
 
 
@@ -90,7 +87,7 @@ def prompt_attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch
     """Sequences laid end to end: ``query`` [total, Hq, 128], ``key`` / ``value`` [total, Hkv, 128] -> [total, Hq, 128].  Sequence
     ``s`` is the tokens ``[cu_seqlens[s], cu_seqlens[s + 1])`` (int32 on the device, ascending) and attends itself alone;
     none is longer than ``max_seqlen``.  Tokens behind the last sequence are left as they were in ``out``."""
-    _check(query, key, value, 3, 1)
+    _check(query, key, value, 3)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be an int32 tensor [sequences + 1]")
     cu_seqlens = _int32(cu_seqlens, (int(cu_seqlens.numel()),), query.device, "cu_seqlens")
@@ -101,11 +98,11 @@ def prompt_attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch
     if n == 0 or max_seqlen == 0:
         return out
     q, k, v = aligned_view(query), aligned_view(key), aligned_view(value)
-    descs = [strided_desc(t.transpose(0, 1).unsqueeze(0)) for t in (q, k, v, out)]
-    refs = [C.byref(d) for d in descs]
-    _launch("tq_prompt_attn_packed", query.device, (n, hq, hkv, int(max_seqlen), int(max_seqlen)),
-            (refs[0], refs[1], refs[2], n, total, hq, hkv, cu_seqlens.data_ptr(), int(max_seqlen),
-             128 ** -0.5 if scale is None else float(scale), int(causal)), (refs[3],))
+    qd, kd, vd, od = (strided_desc(t.transpose(0, 1).unsqueeze(0)) for t in (q, k, v, out))
+    ws, need = _workspace(query.device, n, hq, hkv, int(max_seqlen), int(max_seqlen))
+    ffi.launch("tq_prompt_attn_packed", query.device, (
+        C.byref(qd), C.byref(kd), C.byref(vd), n, total, hq, hkv, cu_seqlens.data_ptr(), int(max_seqlen),
+        _SCALE if scale is None else float(scale), int(causal), None if ws is None else ws.data_ptr(), need, C.byref(od)))
     return out
 
 
