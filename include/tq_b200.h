@@ -249,7 +249,8 @@ int32_t tq_cache_select_rows(tq_ctx *ctx, const tq_cache_desc *src, const tq_cac
  * (stride_b unused); sequence s is the tokens [cu_seqlens[s], cu_seqlens[s + 1]) (device int32 [n_seqs + 1], ascending,
  * not above total), of at most max_seqlen tokens; tokens beyond that, and those behind the last sequence, are left as
  * they were in out.
- * tq_prompt_status: synchronises with the current device; 0, or 1 when a kernel's bounded wait ran out (sticky). */
+ * tq_prompt_status: synchronises with the current device; 0; 1 when a kernel's bounded wait ran out, 2 when its
+ * shared memory was not laid out as it needs (sticky). */
 size_t tq_prompt_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv);
 int32_t tq_prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int32_t batch,
                        int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv, const int32_t *seq_start, float scale,

@@ -58,6 +58,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {  
         "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {  // tmem_st_wait before anybody reads them
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 // (the registers are named so that nothing reads them ahead of the wait)
 __device__ __forceinline__ void tmem_ld_wait(uint32_t *r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n"
@@ -91,6 +98,24 @@ __device__ __forceinline__ float exp2_hw(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^x of two numbers without the unit that exp2_hw shares with the whole SM quarter (16 results a clock and SM): the integer nearest to x goes into
+// the exponent field, 2 to the rest in [-1/2, 1/2] is the cubic of least relative error (found by Remez exchange; 7.5e-5 = 2^-13.7).
+// What is below 2^-125 (-inf too) gives 2^-125: the exponent field does not run over.
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float &p, float &q) {
+    float a, b;
+    f32x2_split(x2, a, b);
+    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(a) : "f"(-125.f));
+    asm("max.NaN.f32 %0, %0, %1;\n" : "+f"(b) : "f"(-125.f));
+    const uint64_t x = f32x2(a, b), magic = f32x2(12582912.f, 12582912.f);  // 1.5 * 2^23: what is added to it is rounded to an integer
+    const uint64_t n = f32x2_add(x, magic);
+    const uint64_t f = f32x2_sub(x, f32x2_add(n, f32x2(-12582912.f, -12582912.f)));
+    uint64_t y = f32x2_fma(f32x2(0.0551716685f, 0.0551716685f), f, f32x2(0.242611125f, 0.242611125f));
+    y = f32x2_fma(y, f, f32x2(0.693260968f, 0.693260968f));
+    y = f32x2_fma(y, f, f32x2(0.999928057f, 0.999928057f));
+    float na, nb, ya, yb;
+    f32x2_split(n, na, nb), f32x2_split(y, ya, yb);
+    p = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(na) << 23)), q = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(nb) << 23));
 }
 // The running maximum that a row's weights are relative to may lag behind the true one by up to 2^kLag: fp16 weights stay below
 // 2^9 and the sums far from overflow, and the accumulator is rescaled a few times a row instead of at every block.

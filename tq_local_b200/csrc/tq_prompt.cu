@@ -10,11 +10,17 @@
 // warps take exponentials.
 //
 // Roles.  Warps 0-3 and 4-7: the softmax of a tile each, one row a thread.  Warp 8: requests the query tiles and the key and value blocks
-// (tensor maps, 128-byte swizzle, a ring of 32 KB slots).  Warp 9: issues the products.  S = Q K^T with both operands in
-// shared memory; the weights go back to TMEM over S as 16-bit pairs and are the A operand of O += P V.
-// TMEM: S of the two tiles, O of the two tiles, 128 columns each.
+// (tensor maps, 128-byte swizzle, a ring of 32 KB slots).  Warps 9 and 10: issue the products of a tile each.  Warp 11: clears values that
+// are outside the sequence.  S = Q K^T with both operands in shared memory; the weights go back to TMEM over S as 16-bit pairs and are the A
+// operand of O += P V.  TMEM: S of the two tiles, O of the two tiles, 128 columns each.
+//
+// What bounds it: 32768 tokens, 32 / 8 heads, bf16, take 7.2 ms on a card at rest (1220 TFLOP/s) and 8.3 ms back to back, where the card's
+// power limit lowers its clock (1060; the library's matrix product falls from 1657 to 1376).  Between steps the tensor core waits for exponentials
+// (16 a clock and SM against 8192 operations: as long as the products) and for the hand-over of logits and weights.
 #include <cuda.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "tq_attn_tc.cuh"
 
@@ -22,11 +28,21 @@ namespace {
 
 __device__ int g_prompt_status;
 
-constexpr int kThreads = 384;
+constexpr int kSoftmax = 256;                    // threads: a row of two tiles each
+constexpr int kThreads = kSoftmax + 128;
 constexpr int kBlock = 128;                      // keys of a block
+// Keys of a step.  The logits of a tile have 128 columns of TMEM, and the weights go over them: with 64 keys a step there are two sets, and the
+// products for one run while the softmax takes the other (8192 tokens, 32 / 8 heads, bf16: 512 us; 597 with 128 keys and one set).
+constexpr int kUnit = 64;
+constexpr int kBuffers = kBlock / kUnit;         // steps whose logits are held at a time, and steps of a block
+// Pairs of exponentials out of eight that the polynomial takes: none 573 us, one 565, two 563, three 566, four 577 (as above, back to back, where the
+// card's power limit holds).
+constexpr int kPolyOf8 = 2;
 constexpr int kSlotBytes = kUmmaTermBytes;       // 128 rows x 128 16-bit values
 constexpr int kSlots = 5;
-constexpr int kSmem = 2 * kSlotBytes + kSlots * kSlotBytes + 1024;
+// two query tiles, the ring, barriers and the TMEM address
+constexpr int kBarsAt = (2 + kSlots) * kSlotBytes, kBars = 2 + 4 + 4 + 2 + 2 * kSlots + 3;
+constexpr int kSmem = kBarsAt + 8 * kBars + 16;
 
 struct PromptArgs {
     void *out;
@@ -54,9 +70,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     tq_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ PromptArgs a) {
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_bars[4 + 4 + 2 * kSlots];
-    __shared__ uint32_t s_tmem;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];  // (swizzle atoms need 1024-byte alignment, and there is no room to spare)
     // ---- this CTA's work: the longest tiles come first
     const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads % a.batch;
     const int item = a.n_items - 1 - blockIdx.x / (a.kv_heads * a.batch);
@@ -67,155 +81,182 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int offset = n_kv - n_q;
     const int start = a.seq_start ? min(max(a.seq_start[b], 0), n_kv) : 0;
     const int block0 = start / kBlock;
-    auto blocks_of = [&](int w) {
+    auto units_of = [&](int w) {
         const int pos = first_pos + w * a.positions;
         if (w >= a.tiles_per_cta || pos >= n_q) return 0;
         const int end = a.causal ? min(n_kv, min(pos + a.positions, n_q) + offset) : n_kv;
-        return end > start ? (end + kBlock - 1) / kBlock - block0 : 0;
+        return end > start ? (end + kUnit - 1) / kUnit - block0 * kBuffers : 0;
     };
-    int nb0 = blocks_of(0), nb1 = blocks_of(1);
-    int first_block = block0;
+    int nu0 = units_of(0), nu1 = units_of(1), first_block = block0;
     if (a.splits > 1) {
-        const int share = (max(nb0, nb1) + a.splits - 1) / a.splits, lo = share * blockIdx.y;
-        first_block += lo, nb0 = min(max(nb0 - lo, 0), share), nb1 = min(max(nb1 - lo, 0), share);
+        const int share = (max(nu0, nu1) + kBuffers * a.splits - 1) / (kBuffers * a.splits) * kBuffers, lo = share * blockIdx.y;  // (whole blocks)
+        first_block += lo / kBuffers, nu0 = min(max(nu0 - lo, 0), share), nu1 = min(max(nu1 - lo, 0), share);
     }
-    const int nb = max(nb0, nb1);
+    const int nu = max(nu0, nu1), nb = (nu + kBuffers - 1) / kBuffers;
 
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = base + 2 * kSlotBytes;
-    const uint32_t bars = smem_u32(s_bars);
-    const uint32_t bar_q = bars, bar_s = bars + 16, bar_p = bars + 32, bar_o = bars + 48, bar_full = bars + 64, bar_empty = bar_full + 8 * kSlots;
+    const uint32_t base = smem_u32(smem_raw), ring = base + 2 * kSlotBytes, bars = base + kBarsAt;
+    uint32_t *const s_tmem = reinterpret_cast<uint32_t *>(smem_raw + kBarsAt + 8 * kBars);
+    if (base & 1023u) {
+        if (threadIdx.x == 0) atomicExch(&g_prompt_status, 2);
+        return;
+    }
+    // q: queries are there; s[tile][unit & 1]: logits are there; p[tile][unit & 1]: weights are there; o[tile]: O += P V is done; full, empty: slots
+    const uint32_t bar_q = bars, bar_s = bars + 16, bar_p = bars + 48, bar_o = bars + 80, bar_full = bars + 96, bar_empty = bar_full + 8 * kSlots, bar_ask = bar_empty + 8 * kSlots, bar_clean = bar_ask + 8;
     const int tid = threadIdx.x, warp = tid >> 5;
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(512));
+    if (warp == kSoftmax / 32 + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     }
     if (tid == 0) {
-        mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1);
-        for (int w = 0; w < 2; ++w) mbar_init(bar_s + 8 * w, 1), mbar_init(bar_p + 8 * w, 128), mbar_init(bar_o + 8 * w, 1);
-        for (int s = 0; s < kSlots; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 1);
+        mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1), mbar_init(bar_ask, 1), mbar_init(bar_clean, 32), mbar_init(bar_clean + 8, 32);
+        for (int i = 0; i < 4; ++i) mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 128);
+        for (int w = 0; w < 2; ++w) mbar_init(bar_o + 8 * w, 1);
+        for (int s = 0; s < kSlots; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
     umma_fence_before();
     __syncthreads();
     umma_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *s_tmem, 0);
     bool lost = false;  // a wait of this thread ran out: it waits for nothing more
     auto wait = [&](uint32_t bar, uint32_t parity) {
         if (!lost && !mbar_wait(bar, parity)) lost = true;
     };
 
-    if (warp >= 8) {
+    auto dirty = [&](int k) { return (first_block + k) * kBlock < start || (first_block + k + 1) * kBlock > n_kv; };
+
+    if (warp >= kSoftmax / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
-        if (warp == 8 && elect_one()) {
+        if (warp == kSoftmax / 32) {
             // ---------------- copies: Q0, K0, Q1, V0, K1, V1, ...
-            const int bb = a.cu_seqlens ? 0 : b;
-            auto load_q = [&](int w) {
-                mbar_expect_tx(bar_q + 8 * w, 256 * a.positions * a.group);
-                for (int x = 0; x < 2; ++x)
-                    load_map(base + w * kSlotBytes + x * kUmmaSlabBytes, &map_q, bar_q + 8 * w, 64 * x, 0, t0 + first_pos + w * a.positions, h, bb);
-            };
-            if (nb0) load_q(0);
-            for (int i = 0; i < 2 * nb; ++i) {
-                const int slot = i % kSlots;
-                wait(bar_empty + 8 * slot, (i / kSlots & 1) ^ 1);
-                const uint32_t bar = bar_full + 8 * slot;
-                mbar_expect_tx(bar, kSlotBytes);
-                for (int x = 0; x < 2; ++x)
-                    load_map(ring + slot * kSlotBytes + x * kUmmaSlabBytes, i & 1 ? &map_v : &map_k, bar, 64 * x, t0 + (first_block + i / 2) * kBlock, h, bb);
-                if (i == 0 && nb1) load_q(1);
-            }
-        } else if (warp == 9) {
-            // ---------------- products
-            const uint32_t instr_s = attn_instr<BF16, false>(a.negate), instr_o = attn_instr<BF16, true>();
-            auto slot_addr = [&](int i) { return ring + i % kSlots * kSlotBytes; };
-            auto wait_full = [&](int i) { wait(bar_full + 8 * (i % kSlots), i / kSlots & 1); };
-            auto scores = [&](int w, int i) {
-                if (elect_one()) {
-                    attn_scores(tmem + 128 * w, base + w * kSlotBytes, slot_addr(i), instr_s);
-                    umma_commit(bar_s + 8 * w);
+            if (elect_one()) {
+                const int bb = a.cu_seqlens ? 0 : b;
+                auto load_q = [&](int w) {
+                    mbar_expect_tx(bar_q + 8 * w, 256 * a.positions * a.group);
+                    for (int x = 0; x < 2; ++x)
+                        load_map(base + w * kSlotBytes + x * kUmmaSlabBytes, &map_q, bar_q + 8 * w, 64 * x, 0, t0 + first_pos + w * a.positions, h, bb);
+                };
+                if (nu0) load_q(0);
+                for (int i = 0; i < 2 * nb; ++i) {
+                    const int slot = i % kSlots;
+                    wait(bar_empty + 8 * slot, (i / kSlots & 1) ^ 1);
+                    const uint32_t bar = bar_full + 8 * slot;
+                    mbar_expect_tx(bar, kSlotBytes);
+                    for (int x = 0; x < 2; ++x)
+                        load_map(ring + slot * kSlotBytes + x * kUmmaSlabBytes, i & 1 ? &map_v : &map_k, bar, 64 * x, t0 + (first_block + i / 2) * kBlock, h, bb);
+                    if (i == 0 && nu1) load_q(1);
                 }
-                __syncwarp();
-            };
-            if (nb) {
-                wait_full(0);
-                if (nb0) wait(bar_q, 0), umma_fence_after(), scores(0, 0);
-                if (nb1) wait(bar_q + 8, 0), umma_fence_after(), scores(1, 0);
-                if (kSlots < 2 * nb && elect_one()) umma_commit(bar_empty);
-                __syncwarp();
             }
-            for (int k = 0; k < nb; ++k) {
-                const int iv = 2 * k + 1, ik = 2 * k + 2;
-                wait_full(iv);
-                // Values that no query sees may hold anything, and 0 * inf is not 0: they become 0.
-                const int j0 = (first_block + k) * kBlock, dirty_lo = start - j0, clean_hi = n_kv - j0;
-                if (dirty_lo > 0 || clean_hi < kBlock) {
-                    for (int i = tid & 31; i < kBlock * 16; i += 32) {
-                        const int row = i >> 4;
-                        if (row < dirty_lo || row >= clean_hi) sts128(slot_addr(iv) + (i & 8) / 8 * kUmmaSlabBytes + row * 128 + (i & 7) * 16, 0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    __syncwarp();
-                }
-                if (k + 1 < nb) wait_full(ik);
+        } else if (warp < kSoftmax / 32 + 3) {
+            // ---------------- products of tile w.  A wait costs a thread some 200 cycles even when there is nothing to wait for; a warp a tile keeps
+            // the tensor core busy with one tile's products meanwhile.
+            const int w = warp - (kSoftmax / 32 + 1), mine = w ? nu1 : nu0;
+            if (elect_one()) {
+                const uint32_t instr_s = attn_instr<BF16, false>(a.negate) - (((kBlock - kUnit) >> 3) << 17), instr_o = attn_instr<BF16, true>();
+                auto slot_addr = [&](int i) { return ring + i % kSlots * kSlotBytes; };
+                auto wait_full = [&](int i) { wait(bar_full + 8 * (i % kSlots), i / kSlots & 1); };
+                constexpr uint32_t kHalf = kUnit * 128;  // bytes of 64 rows in a slab
+                auto scores = [&](int u) {               // S[u % kBuffers] = Q K_u^T
+                    const uint64_t q = umma_desc<false>(base + w * kSlotBytes), k = umma_desc<false>(slot_addr(2 * (u / kBuffers)) + u % kBuffers * kHalf);
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const int mine = w ? nb1 : nb0;
-                    if (k >= mine) continue;
-                    wait(bar_p + 8 * w, k & 1);
-                    umma_fence_after();
-                    if (elect_one()) {
-                        attn_values(tmem + 256 + 128 * w, tmem + 128 * w, slot_addr(iv), instr_o, k > 0);
-                        if (k + 1 == mine) umma_commit(bar_o + 8 * w);
+                    for (uint32_t s = 0; s < 8; ++s) {
+                        const uint32_t step = ((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4;
+                        umma_ss(tmem + 128 * w + kUnit * (u % kBuffers), q + step, k + step, instr_s, s > 0);
                     }
-                    __syncwarp();
-                    if (k + 1 < mine) scores(w, ik);
+                    umma_commit(bar_s + 16 * w + 8 * (u % kBuffers));
+                };
+                auto values = [&](int u) {  // O += P[u % kBuffers] V_u
+                    const uint64_t v = umma_desc<true>(slot_addr(2 * (u / kBuffers) + 1) + u % kBuffers * kHalf);
+#pragma unroll
+                    for (uint32_t s = 0; s < kUnit / 16; ++s)
+                        umma_f16(tmem + 256 + 128 * w, tmem + 128 * w + kUnit * (u % kBuffers) + 8 * s, v + ((s * 16 * 128) >> 4), instr_o, u > 0 || s > 0);
+                    umma_commit(bar_o + 8 * w);
+                };
+                auto release = [&](int i) {  // (a slot that is filled again; the other tile's thread does the same)
+                    if (i + kSlots < 2 * nb) umma_commit(bar_empty + 8 * (i % kSlots));
+                };
+                if (nb) {
+                    wait_full(0);
+                    if (mine) wait(bar_q + 8 * w, 0), scores(0);
+                    if (kBuffers > 1 && mine > 1) scores(1);
+                    release(0);
                 }
-                if (iv + kSlots < 2 * nb && elect_one()) {  // (a slot that is filled again)
-                    umma_commit(bar_empty + 8 * (iv % kSlots));
-                    if (ik + kSlots < 2 * nb) umma_commit(bar_empty + 8 * (ik % kSlots));
+                for (int k = 0; k < nb; ++k) {
+                    wait_full(2 * k + 1);
+                    if (dirty(k)) {
+                        if (w == 0) mbar_arrive_one(bar_ask);
+                        wait(bar_clean + (k ? 8 : 0), 0);
+                    }
+                    if (k + 1 < nb) wait_full(2 * k + 2);
+#pragma unroll
+                    for (int e = 0; e < kBuffers; ++e) {
+                        const int u = kBuffers * k + e;
+                        if (u >= mine) continue;
+                        wait(bar_p + 16 * w + 8 * e, k & 1);
+                        umma_fence_after();
+                        values(u);
+                        if (u + kBuffers < mine) scores(u + kBuffers);  // (over the weights that were multiplied just before)
+                    }
+                    release(2 * k + 1), release(2 * k + 2);
                 }
+            }
+        } else {
+            // ---------------- values that no query sees may hold anything, and 0 * inf is not 0: they become 0 (in the first block and the last)
+            for (int k = 0, asked = 0; k < nb; ++k) {
+                if (!dirty(k)) continue;
+                const int slot = (2 * k + 1) % kSlots, j0 = (first_block + k) * kBlock;
+                wait(bar_ask, asked++ & 1);
                 __syncwarp();
+                for (int i = tid & 31; i < kBlock * 16; i += 32) {
+                    const int row = i >> 4;
+                    if (row < start - j0 || row >= n_kv - j0) sts128(ring + slot * kSlotBytes + (i & 8) / 8 * kUmmaSlabBytes + row * 128 + (i & 7) * 16, 0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                mbar_arrive_one(bar_clean + (k ? 8 : 0));
             }
         }
     } else {
         // ---------------- softmax of tile w, one row a thread
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
-        const int w = warp >> 2, row = tid & 127, mine = w ? nb1 : nb0;
+        const int w = warp >> 2, row = tid & 127, mine = w ? nu1 : nu0;
         const int pos = first_pos + w * a.positions + row / a.group;
         const bool live = w < a.tiles_per_cta && row < a.positions * a.group && pos < n_q;
         const int limit = a.causal ? min(n_kv, pos + offset + 1) : n_kv;  // keys [start, limit)
         const int tile_limit = a.causal ? min(n_kv, first_pos + w * a.positions + offset + 1) : n_kv;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_s = tmem + 128 * w + lanes, t_o = tmem + 256 + 128 * w + lanes;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_o = tmem + 256 + 128 * w + lanes;
         const float c = a.scale_log2;
         float m_ref = -INFINITY;
         uint64_t sum[2] = {0, 0};
-        for (int k = 0; k < mine; ++k) {
-            wait(bar_s + 8 * w, k & 1);
+        for (int u = 0; u < mine; ++u) {
+            const int e = u % kBuffers;
+            const uint32_t t_s = tmem + 128 * w + kUnit * e + lanes;
+            wait(bar_s + 16 * w + 8 * e, u / kBuffers & 1);
             __syncwarp();
             umma_fence_after();
-            uint32_t s[128];
+            uint32_t s[kUnit];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s + 32 * i);
+            for (int i = 0; i < kUnit; i += 32) tmem_ld32(t_s + i, s + i);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld_wait(s + 32 * i);
-            const int j0 = (first_block + k) * kBlock;
-            if (j0 < start || j0 + kBlock > tile_limit) {
+            for (int i = 0; i < kUnit; i += 32) tmem_ld_wait(s + i);
+            const int j0 = first_block * kBlock + u * kUnit;
+            const bool masked = j0 < start || j0 + kUnit > tile_limit;
+            if (masked) {
                 const int lo = start - j0, hi = limit - j0;
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
+                for (int i = 0; i < kUnit; ++i)
                     if (i < lo || i >= hi) s[i] = 0xff800000u;
             }
             float top[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) top[i] = max3(__uint_as_float(s[i]), __uint_as_float(s[i + 4]), __uint_as_float(s[i + 8]));
 #pragma unroll
-            for (int i = 12; i < 124; i += 8)
+            for (int i = 12; i < kUnit - 4; i += 8)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
-            float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            peak = fmaxf(peak, max3(__uint_as_float(s[124]), __uint_as_float(s[125]), fmaxf(__uint_as_float(s[126]), __uint_as_float(s[127]))));
-            if (k == 0) {
+                for (int x = 0; x < 4; ++x) top[x] = max3(top[x], __uint_as_float(s[i + x]), __uint_as_float(s[i + x + 4]));
+            const float last = max3(__uint_as_float(s[kUnit - 4]), __uint_as_float(s[kUnit - 3]), fmaxf(__uint_as_float(s[kUnit - 2]), __uint_as_float(s[kUnit - 1])));
+            const float peak = max3(max3(top[0], top[1], top[2]), top[3], last);
+            if (u == 0) {
                 m_ref = peak;
             } else {
                 const bool raise = live && (peak - m_ref) * c > kLag;
@@ -224,8 +265,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (raise) keep = exp2_hw((m_ref - peak) * c), m_ref = peak;
                     const uint64_t keep2 = f32x2(keep, keep);
                     sum[0] = f32x2_mul(sum[0], keep2), sum[1] = f32x2_mul(sum[1], keep2);
+                    wait(bar_o + 8 * w, (u - 1) & 1);  // the values of the unit before; those of this one wait for its weights
+                    __syncwarp();
+                    umma_fence_after();
 #pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {  // (S_k was multiplied after O_(k-1): nobody else touches O now)
+                    for (int i = 0; i < 4; ++i) {
                         uint32_t o[32];
                         tmem_ld32(t_o + 32 * i, o);
                         tmem_ld_wait(o);
@@ -237,29 +281,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const float shift = m_ref == -INFINITY ? 0.f : -m_ref * c;
             const uint64_t c2 = f32x2(c, c), shift2 = f32x2(shift, shift);
+            auto weights = [&](auto poly) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t p[32];
+                for (int part = 0; part < kUnit; part += 64) {
+                    uint32_t p[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    float x, y;
-                    f32x2_split(f32x2_fma(f32x2(__uint_as_float(s[64 * half + 2 * i]), __uint_as_float(s[64 * half + 2 * i + 1])), c2, shift2), x, y);
-                    x = exp2_hw(x), y = exp2_hw(y);
-                    sum[i & 1] = f32x2_add(sum[i & 1], f32x2(x, y));
-                    p[i] = pack16<BF16>(x, y);
+                    for (int i = 0; i < 32; ++i) {
+                        const uint64_t x2 = f32x2_fma(f32x2(__uint_as_float(s[part + 2 * i]), __uint_as_float(s[part + 2 * i + 1])), c2, shift2);
+                        float x, y;
+                        if (decltype(poly)::value && i % 8 < kPolyOf8) {
+                            exp2_poly(x2, x, y);
+                        } else {
+                            f32x2_split(x2, x, y);
+                            x = exp2_hw(x), y = exp2_hw(y);
+                        }
+                        sum[i & 1] = f32x2_add(sum[i & 1], f32x2(x, y));
+                        p[i] = pack16<BF16>(x, y);
+                    }
+                    tmem_st32(t_s + part / 2, p);
                 }
-                tmem_st32(t_s + 32 * half, p);
-            }
+            };
+            if (masked) weights(std::false_type());  // (a hidden key's weight is 0)
+            else weights(std::true_type());
             tmem_st_wait();
             umma_fence_before();
-            mbar_arrive_one(bar_p + 8 * w);
+            mbar_arrive_one(bar_p + 16 * w + 8 * e);
         }
         // ---------------- the tile's rows
         float l0, l1;
         f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
         const float l = l0 + l1;
-        if (mine) {
-            wait(bar_o + 8 * w, 0);
+        if (mine) {  // (the unit before the last as well: the barrier says which of two is done only to who knows the one before)
+            if (mine > 1) wait(bar_o + 8 * w, mine & 1);
+            wait(bar_o + 8 * w, (mine - 1) & 1);
             __syncwarp();
             umma_fence_after();
         }
@@ -307,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lost) atomicExch(&g_prompt_status, 1);
     umma_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kSoftmax / 32 + 1) {
         umma_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
     }

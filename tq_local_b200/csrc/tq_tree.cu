@@ -564,6 +564,8 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             // ---- this piece of the tile's rows
             float l0, l1;
             f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
+            // (the block before the last as well: the barrier says which of two is done only to who knows the one before)
+            if (g.k_end - g.k > 1) wait(bar_o, n & 1);
             wait(bar_o, (n - 1) & 1);
             __syncwarp();
             umma_fence_after();

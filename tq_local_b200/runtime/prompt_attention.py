@@ -112,7 +112,8 @@ def raise_on_status(device: torch.device, where: str) -> None:
     with torch.cuda.device(device):
         ffi.check(ffi.lib().tq_prompt_status(C.byref(v)), "tq_prompt_status")
     if v.value:
-        raise ffi.TQError(f"{where}: a prompt attention kernel's wait ran out; its outputs are not valid")
+        raise ffi.TQError(f"{where}: a prompt attention kernel gave up (status {v.value}: 1 a wait ran out, 2 its shared memory did not fit); "
+                          "its outputs are not valid")
 
 
 def _takes(query, key, attention_mask, is_causal, dropout, kwargs) -> bool:
