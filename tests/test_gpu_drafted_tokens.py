@@ -189,6 +189,18 @@ def test_extreme_norms():
     check(store.tree_attn(q), reference(store, q, 391))
 
 
+@pytest.mark.parametrize("b,hkv,n,t", [(3, 8, 4500, 3), (2, 16, 3001, 64), (40, 8, 200, 1), (1, 2, 30_000, 40)])
+def test_many_blocks_and_many_rows_a_cta(b, hkv, n, t):
+    """More blocks than SMs: a CTA goes through several, and from one row of the cache to the next."""
+    store = make_store(4, True, b, hkv, n + t, seed=b)
+    lengths = torch.randint(0, n + 1, (b,), generator=torch.Generator().manual_seed(b), dtype=torch.int32).cuda()
+    q, mask = queries(b, 2 * hkv, t, F16), random_tree(b, t, 9)
+    for _ in range(20):
+        out = store.tree_attn(q, words(mask), lengths=lengths)
+    check(out, reference(store, q, n, mask, lengths))
+    assert store.codec.device_status() == 0
+
+
 def test_query_layouts_and_given_output():
     store = make_store(4, True, 2, 2, 300)
     q = queries(2, 8, 10, BF16)

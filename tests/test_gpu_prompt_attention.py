@@ -187,6 +187,18 @@ def test_long_keys_few_queries_and_equal_runs():
             assert torch.equal(out, prompt_attention(q, k, v, seq_start=s))
 
 
+def test_many_tiles():
+    """More tiles than SMs, again and again."""
+    from tq_local_b200.runtime.prompt_attention import prompt_attention, raise_on_status
+
+    for b, hq, hkv, n in ((1, 8, 8, 4000), (6, 16, 4, 700), (60, 4, 1, 130)):
+        q, k, v = make(b, hq, hkv, n, n, BF16, n)
+        for _ in range(30):
+            out = prompt_attention(q, k, v)
+        check(out[:2], *reference(q[:2], k[:2], v[:2]))
+    raise_on_status(q.device, "test")
+
+
 def test_other_stream_and_recorded():
     from tq_local_b200.runtime.prompt_attention import prompt_attention, raise_on_status
 

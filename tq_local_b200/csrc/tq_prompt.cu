@@ -305,14 +305,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             else weights(std::true_type());
             tmem_st_wait();
             umma_fence_before();
+            // (the wait for the last values tells them from those before only if these are known to be done)
+            if (u && u + 1 == mine) wait(bar_o + 8 * w, (u - 1) & 1);
             mbar_arrive_one(bar_p + 16 * w + 8 * e);
         }
         // ---------------- the tile's rows
         float l0, l1;
         f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
         const float l = l0 + l1;
-        if (mine) {  // (the unit before the last as well: the barrier says which of two is done only to who knows the one before)
-            if (mine > 1) wait(bar_o + 8 * w, mine & 1);
+        if (mine) {
             wait(bar_o + 8 * w, (mine - 1) & 1);
             __syncwarp();
             umma_fence_after();

@@ -22,7 +22,8 @@
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kSoftmaxWarps = 4, kOperandWarps = 16;  // and four more, of which one issues the products
+constexpr int kThreads = 32 * (kSoftmaxWarps + kOperandWarps + 4);
 constexpr int kBlock = 128;  // tokens of a block
 
 struct TreeArgs {
@@ -45,6 +46,9 @@ struct TreeArgs {
     int ctas;
     int *error_flag;
 };
+
+// Where a coordinate lies in the operands and in O: the second and third eight of the last two quarters change places (see the stores below).
+__device__ __forceinline__ int turned(int quarter, int eight) { return eight ^ (quarter & 2); }
 
 struct Entry {
     int start, history;
@@ -210,30 +214,28 @@ template <typename T, bool QJL> __global__ void __launch_bounds__(kRowThreads, 1
         if (mine) {
             uint4 *dst = reinterpret_cast<uint4 *>(a.qop + r * kWide + 128 * i + 32 * part);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) dst[turned(part, e)] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
     }
     tile.finish(a.error_flag);
 }
 
 // ---------------------------------------------------------------------------------------------------- attention
+// Shared memory: two stages of keys and of values, one of signs, and the tables of centre pairs.  A slot of a table holds its pair once per
+// lane, so that every lane reads its own bank.
 template <int KB, int VB, bool QJL> struct Layout {
-    static constexpr int kStage = (QJL ? 3 : 2) * kUmmaTermBytes;  // keys, values, signs of a block
-    // A slot of a table holds one pair of centres once per lane, so that lanes read their own banks; half as often where 256 slots and
-    // two stages with signs leave no room (two lanes then share a bank).
-    static constexpr int kKeySlot = 128, kValueSlot = QJL && VB == 4 ? 64 : 128;
-    static constexpr int kKeyTable = (1 << 2 * KB) * kKeySlot, kValueTable = (1 << 2 * VB) * kValueSlot;
-    static constexpr int kBytes = 2 * kStage + kKeyTable + kValueTable + 1024;
+    static constexpr int kKeys = 0, kValues = 2 * kUmmaTermBytes, kSigns = 4 * kUmmaTermBytes;
+    static constexpr int kKeyTable = kSigns + (QJL ? kUmmaTermBytes : 0), kValueTable = kKeyTable + 128 * (1 << 2 * KB);
+    static constexpr int kBytes = kValueTable + 128 * (1 << 2 * VB) + 1024;
 };
 
 // Word i of the operand from 32 codes in BITS words (and one that is not looked at): two neighbouring codes by one look-up, times the norm.
-template <int BITS, int SLOT> __device__ __forceinline__ uint32_t centre_pair(const uint32_t *words, int i, uint32_t lane_addr, uint32_t norm2) {
-    constexpr int kShift = SLOT == 128 ? 7 : 6;
-    constexpr uint32_t kMask = ((1u << 2 * BITS) - 1u) << kShift;
+template <int BITS> __device__ __forceinline__ uint32_t centre_pair(const uint32_t *words, int i, uint32_t lane_addr, uint32_t norm2) {
+    constexpr uint32_t kMask = ((1u << 2 * BITS) - 1u) << 7;
     const int bit = 2 * BITS * i, w = bit >> 5, sh = bit & 31;
     uint32_t x;
-    if (sh + 2 * BITS > 32) x = __funnelshift_r(words[w], words[w + 1], sh) << kShift;
-    else x = sh >= kShift ? words[w] >> (sh - kShift) : words[w] << (kShift - sh);
+    if (sh + 2 * BITS > 32) x = __funnelshift_r(words[w], words[w + 1], sh) << 7;
+    else x = sh >= 7 ? words[w] >> (sh - 7) : words[w] << (7 - sh);
     uint32_t v;
     asm("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"((x & kMask) + lane_addr));
     const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&norm2));
@@ -255,39 +257,38 @@ __device__ __forceinline__ uint32_t seen_word(uint64_t mask, int chain_end, int 
 template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 1) tq_tree_kernel(const __grid_constant__ TreeArgs a) {
     using L = Layout<KB, VB, QJL>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 2 + 2 + 1 + 1];
+    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 2 + 1 + 1];
     __shared__ uint32_t s_tmem;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t table_k = base + 2 * L::kStage, table_v = table_k + L::kKeyTable;
     const uint32_t bars = smem_u32(s_bars);
-    // full: operands are there; free: the products that read them are done; s: logits are there; p: weights are there; o: O += P V is done; q: queries are there
-    const uint32_t bar_kfull = bars, bar_vfull = bars + 16, bar_kfree = bars + 32, bar_vfree = bars + 48, bar_s = bars + 64, bar_p = bars + 80, bar_o = bars + 96, bar_q = bars + 104;
+    // full: operands are there; kfree, vfree: the products that read keys and signs, or values, are done; s: logits are there; p: weights are there;
+    // o: O += P V is done; q: queries are there
+    const uint32_t bar_full = bars, bar_kfree = bars + 16, bar_vfree = bars + 32, bar_s = bars + 48, bar_p = bars + 64, bar_o = bars + 80, bar_q = bars + 88;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (warp == 12) {
+    constexpr int kProducts = kSoftmaxWarps + kOperandWarps;
+    const int row_warps = (a.rows + 31) >> 5;  // warps of the softmax that have rows (the others' rows of S and O are what they are)
+    if (warp == kProducts) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_kfull + 8 * i, 256), mbar_init(bar_vfull + 8 * i, 256);
-            mbar_init(bar_kfree + 8 * i, 1), mbar_init(bar_vfree + 8 * i, 1);
-            mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 128);
+            mbar_init(bar_full + 8 * i, 16 * kOperandWarps), mbar_init(bar_kfree + 8 * i, 1), mbar_init(bar_vfree + 8 * i, 1);
+            mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 32 * row_warps);
         }
-        mbar_init(bar_o, 1), mbar_init(bar_q, 128);
+        mbar_init(bar_o, 1), mbar_init(bar_q, 32 * row_warps);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     {
         const float ck = a.centers_k[lane & 15], cv = a.centers_v[lane & 15];
-        auto fill = [&](uint32_t table, int slot, int bits, float centre) {
-            const int copies = slot / 4;
-            for (int i = tid; i < (copies << 2 * bits); i += kThreads) {  // (whole warps)
-                const int e = i / copies;
+        auto fill = [&](uint32_t table, int bits, float centre) {
+            for (int e = warp; e < 1 << 2 * bits; e += kThreads / 32) {
                 const float lo = __shfl_sync(0xffffffffu, centre, e & ((1 << bits) - 1)), hi = __shfl_sync(0xffffffffu, centre, e >> bits);
-                asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(table + 4 * i), "r"(half2_bits(lo, hi)) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(table + 128 * e + 4 * lane), "r"(half2_bits(lo, hi)) : "memory");
             }
         };
-        fill(table_k, L::kKeySlot, KB, ck);
-        fill(table_v, L::kValueSlot, VB, cv);
+        fill(base + L::kKeyTable, KB, ck);
+        fill(base + L::kValueTable, VB, cv);
     }
     umma_fence_before();
     __syncthreads();
@@ -333,27 +334,23 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         if (!lost && !mbar_wait(bar, parity)) lost = true;
     };
 
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
-        if (warp == 12) {
-            // ---------------- products; n counts blocks since the kernel began
+    if (warp >= kProducts) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+        if (warp == kProducts && elect_one()) {
+            // ---------------- products, by one thread; n counts blocks since the kernel began
             constexpr uint32_t instr_s = umma_instr<false>(), instr_o = umma_instr<true>();
             auto scores = [&](uint32_t n) {
-                wait(bar_kfull + 8 * (n & 1), n >> 1 & 1);
+                wait(bar_full + 8 * (n & 1), n >> 1 & 1);
                 umma_fence_after();
-                if (elect_one()) {
-                    const uint32_t stage = base + (n & 1) * L::kStage, d = tmem + 128 * (n & 1);
 #pragma unroll
-                    for (int part = 0; part < (QJL ? 2 : 1); ++part) {
-                        const uint64_t desc = umma_desc<false>(stage + 2 * part * kUmmaTermBytes);
+                for (int part = 0; part < (QJL ? 2 : 1); ++part) {
+                    const uint64_t desc = umma_desc<false>(base + (part ? L::kSigns : L::kKeys + (n & 1) * kUmmaTermBytes));
 #pragma unroll
-                        for (uint32_t s = 0; s < 8; ++s)
-                            umma_f16(d, t_q + 64 * part + 8 * s, desc + (((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4), instr_s, part | (s > 0));
-                    }
-                    umma_commit(bar_s + 8 * (n & 1));
-                    umma_commit(bar_kfree + 8 * (n & 1));
+                    for (uint32_t s = 0; s < 8; ++s)
+                        umma_f16(tmem + 128 * (n & 1), t_q + 64 * part + 8 * s, desc + (((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4), instr_s, part | (s > 0));
                 }
-                __syncwarp();
+                umma_commit(bar_s + 8 * (n & 1));
+                umma_commit(bar_kfree + 8 * (n & 1));
             };
             uint32_t n = 0, segment = 0;
             while (flat < flat_end) {
@@ -363,111 +360,94 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                 scores(n);
                 for (bool first = true; n < end; ++n, first = false) {
                     if (n + 1 < end) scores(n + 1);
-                    wait(bar_vfull + 8 * (n & 1), n >> 1 & 1);
                     wait(bar_p + 8 * (n & 1), n >> 1 & 1);
                     umma_fence_after();
-                    if (elect_one()) {
-                        attn_values(t_o, tmem + 128 * (n & 1), base + (n & 1) * L::kStage + kUmmaTermBytes, instr_o, !first);
-                        umma_commit(bar_vfree + 8 * (n & 1));
-                        umma_commit(bar_o);
-                    }
-                    __syncwarp();
+                    attn_values(t_o, tmem + 128 * (n & 1), base + L::kValues + (n & 1) * kUmmaTermBytes, instr_o, !first);
+                    umma_commit(bar_vfree + 8 * (n & 1));
+                    umma_commit(bar_o);
                 }
             }
         }
-    } else if (warp >= 4) {
-        // ---------------- operands: half of a token's coordinates a thread
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
-        const int row = tid & 127, half = (tid - 128) >> 7;
-        uint32_t kw[2 * KB + 1], vw[2 * VB + 1], sw[2];
-        uint16_t kn, vn, rn;
-        kw[2 * KB] = vw[2 * VB] = 0;
+    } else if (warp >= kSoftmaxWarps) {
+        // ---------------- operands.  Half of the warps take the even blocks, half the odd ones: a thread's loads have two blocks' time to arrive, and
+        // none are on their way when it fences its stores (the fence would wait for them).  A quarter of two tokens' coordinates a thread, four
+        // lanes to a token, so that a load covers whole lines.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+        const uint32_t half = (uint32_t)(warp - kSoftmaxWarps) / (kOperandWarps / 2);
+        const int quarter = lane & 3, row0 = 16 * ((warp - kSoftmaxWarps) % (kOperandWarps / 2)) + (lane >> 2);  // and row0 + 8
+        uint32_t kw[2][KB + 1] = {}, vw[2][VB + 1] = {}, sw[2] = {};
+        uint16_t kn[2], vn[2], rn[2];
         Segment g;
         int k = 0, k_end = 0;
-        auto words = [&](const uint8_t *src, int n, uint32_t *w) {
-            if (n % 4 == 0) {
-                for (int i = 0; i < n; i += 4) {
-                    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(src) + i / 4);
-                    w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
-                }
+        uint32_t n = 0;  // blocks since the kernel began
+        auto words = [&](const uint8_t *src, auto count, uint32_t *w) {
+            constexpr int n = decltype(count)::value;
+            if constexpr (n == 4) {
+                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(src));
+                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+            } else if constexpr (n == 2) {
+                const uint2 x = __ldg(reinterpret_cast<const uint2 *>(src));
+                w[0] = x.x, w[1] = x.y;
             } else {
-                for (int i = 0; i < n; i += 2) {
-                    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(src) + i / 2);
-                    w[i] = x.x, w[i + 1] = x.y;
-                }
+#pragma unroll
+                for (int i = 0; i < n; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
             }
         };
-        auto fetch = [&]() {  // the next block's token of this thread; false behind the last
+        auto next_block = [&]() {  // false behind the last
             if (k == k_end) {
                 if (flat >= flat_end) return false;
                 g = next_segment(), k = g.k, k_end = g.k_end;
             }
-            const int v = k * kBlock + row;
-            ++k;
-            kn = vn = rn = 0;
-            if (v < g.history + a.nodes) {
-                const int64_t t = g.b * a.cache_sb + g.h * a.cache_sh + (v < g.history ? g.start + v : a.tree_start + v - g.history);
-                words(a.k_codes + t * 16 * KB + 8 * KB * half, 2 * KB, kw);
-                words(a.v_codes + t * 16 * VB + 8 * VB * half, 2 * VB, vw);
-                kn = __ldg(a.k_norms + t), vn = __ldg(a.v_norms + t);
-                if (QJL) words(a.k_signs + t * 16 + 8 * half, 2, sw), rn = __ldg(a.k_rnorms + t);
-            }
             return true;
         };
-        const uint32_t lane_k = table_k + 4 * (lane & (L::kKeySlot / 4 - 1)), lane_v = table_v + 4 * (lane & (L::kValueSlot / 4 - 1));
-        const uint32_t my_row = base + half * kUmmaSlabBytes + (row >> 3) * 1024 + (row & 7) * 128, turn = row & 7;
-        for (int i = 0; i < 2 * KB; ++i) kw[i] = 0;
-        for (int i = 0; i < 2 * VB; ++i) vw[i] = 0;
-        sw[0] = sw[1] = 0;
-        bool more = fetch();
-        for (uint32_t n = 0; more; ++n) {
-            const uint32_t dst = my_row + (n & 1) * L::kStage, parity = (n >> 1 & 1) ^ 1;
-            wait(bar_kfree + 8 * (n & 1), parity);
-            const uint32_t kn2 = kn * 0x10001u, vn2 = vn * 0x10001u, rn2 = (rn * 0x10001u) ^ 0x80008000u;
+        auto fetch = [&]() {  // the block's tokens of this thread
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                uint32_t o[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = centre_pair<KB, L::kKeySlot>(kw, 4 * c + i, lane_k, kn2);
-                sts128(dst + ((c ^ turn) << 4), o[0], o[1], o[2], o[3]);
-            }
-            if (QJL) {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {  // signs p and p + 16 of a word; a set bit is +
-                        const int p = (c & 3) * 4 + i;
-                        o[i] = ((sw[c >> 2] << (15 - p)) & 0x80008000u) ^ rn2;
-                    }
-                    sts128(dst + 2 * kUmmaTermBytes + ((c ^ turn) << 4), o[0], o[1], o[2], o[3]);
+            for (int i = 0; i < 2; ++i) {
+                const int v = k * kBlock + row0 + 8 * i;
+                kn[i] = vn[i] = rn[i] = 0;
+                if (v < g.history + a.nodes) {
+                    const int64_t t = g.b * a.cache_sb + g.h * a.cache_sh + (v < g.history ? g.start + v : a.tree_start + v - g.history);
+                    words(a.k_codes + t * 16 * KB + 4 * KB * quarter, std::integral_constant<int, KB>(), kw[i]);
+                    words(a.v_codes + t * 16 * VB + 4 * VB * quarter, std::integral_constant<int, VB>(), vw[i]);
+                    kn[i] = __ldg(a.k_norms + t), vn[i] = __ldg(a.v_norms + t);
+                    if (QJL) sw[i] = __ldg(reinterpret_cast<const uint32_t *>(a.k_signs + t * 16) + quarter), rn[i] = __ldg(a.k_rnorms + t);
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            mbar_arrive_one(bar_kfull + 8 * (n & 1));
-            uint32_t vnow[2 * VB + 1];
+        };
+        const uint32_t lane_k = base + L::kKeyTable + 4 * lane, lane_v = base + L::kValueTable + 4 * lane;
+        // Eight lanes store two tokens' quarters: with the last two quarters' eights turned, to eight different banks of 16 bytes.
+        const uint32_t turn = (quarter & 1) * 4 ^ (quarter & 2) ^ (row0 & 7), stage = half * kUmmaTermBytes;
+        const uint32_t my_row = base + (quarter >> 1) * kUmmaSlabBytes + (row0 >> 3) * 1024 + (row0 & 7) * 128;
+        auto put = [&](uint32_t at, auto word) {  // word(i, j): word j of the 16 of token i
 #pragma unroll
-            for (int i = 0; i <= 2 * VB; ++i) vnow[i] = vw[i];
-            more = fetch();
-            wait(bar_vfree + 8 * (n & 1), parity);
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                uint32_t o[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = centre_pair<VB, L::kValueSlot>(vnow, 4 * c + i, lane_v, vn2);
-                sts128(dst + kUmmaTermBytes + ((c ^ turn) << 4), o[0], o[1], o[2], o[3]);
+                for (int c = 0; c < 4; ++c)
+                    sts128(my_row + at + 1024 * i + ((c ^ turn) << 4), word(i, 4 * c), word(i, 4 * c + 1), word(i, 4 * c + 2), word(i, 4 * c + 3));
+        };
+        for (; next_block(); ++n, ++k) {
+            if ((n & 1) != half) continue;
+            fetch();
+            if (n > 1) wait(bar_vfree + 8 * half, (n >> 1 & 1) ^ 1);  // (two blocks ago; its logits came before)
+            put(L::kKeys + stage, [&](int i, int j) { return centre_pair<KB>(kw[i], j, lane_k, kn[i] * 0x10001u); });
+            put(L::kValues + stage, [&](int i, int j) { return centre_pair<VB>(vw[i], j, lane_v, vn[i] * 0x10001u); });
+            if (QJL) {
+                if (n) wait(bar_kfree + 8 * (half ^ 1), (n - 1) >> 1 & 1);  // (the signs have one stage)
+                put(L::kSigns, [&](int i, int j) {  // signs j and j + 16 of a word; a set bit is +
+                    return ((sw[i] << (15 - j)) & 0x80008000u) ^ (rn[i] * 0x10001u) ^ 0x80008000u;
+                });
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            mbar_arrive_one(bar_vfull + 8 * (n & 1));
+            mbar_arrive_one(bar_full + 8 * half);
         }
     } else {
         // ---------------- softmax, one row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
         const int row = tid;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         constexpr int kWide = QJL ? 256 : 128;
         uint32_t n = 0;
-        while (flat < flat_end) {
+        if (warp < row_warps) while (flat < flat_end) {
             const Segment g = next_segment();
             const int node = g.t * a.positions + row / a.group;
             const bool live = row < a.rows && node < a.nodes;
@@ -559,13 +539,13 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                 }
                 tmem_st_wait();
                 umma_fence_before();
+                // (the wait for the last values tells them from those before only if these are known to be done)
+                if (k > g.k && k + 1 == g.k_end) wait(bar_o, (n - 1) & 1);
                 mbar_arrive_one(bar_p + 8 * (n & 1));
             }
             // ---- this piece of the tile's rows
             float l0, l1;
             f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
-            // (the block before the last as well: the barrier says which of two is done only to who knows the one before)
-            if (g.k_end - g.k > 1) wait(bar_o, n & 1);
             wait(bar_o, (n - 1) & 1);
             __syncwarp();
             umma_fence_after();
@@ -587,7 +567,7 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
     if (lost) atomicExch(a.error_flag, 8);
     umma_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kProducts) {
         umma_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
     }
@@ -595,55 +575,85 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
 
 // ---------------------------------------------------------------------------------------------------- join
 // Merges a row's pieces, brings its largest coordinate to [2^13, 2^14) for the fp16 terms, un-rotates and rounds.
+// Where a CTA has few rows, the pieces of a row are shared out: thread (slot, part) takes every `groups`-th piece of row slot % rows.
 template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_join_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows, int per_cta) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t s_bars[2];
     __shared__ uint32_t s_tmem;
     __shared__ float s_most[4][128];
+    __shared__ float2 s_ml[128];
     const uint32_t images = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    float4 *const s_part = reinterpret_cast<float4 *>(smem_raw + (images - smem_u32(smem_raw)) + kUmmaImageBytes);  // [slot][33]
     RowTile tile;
     tile.start(&s_tmem, s_bars, images, a.image_v, nullptr);
-    const int row = threadIdx.x & 127, part = threadIdx.x >> 7;
+    const int slot = threadIdx.x & 127, part = threadIdx.x >> 7;
     const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
+    int rows = 8;
+    while (rows < per_cta) rows *= 2;
+    const int groups = kUmmaRows / rows, row = slot & (rows - 1), group = slot / rows;
     const int64_t r = (int64_t)blockIdx.x * per_cta + row;
     RowPlace p = {};
     if (row < per_cta && r < n_rows) p = place_of(a, r, n_rows);
     tq_grid_dependency_wait();
     float o[32] = {};
+    float m = -INFINITY, l = 0.f;
     if (p.live) {
         const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
         const int history = entry_of(a, p.b).history, t = (int)(p.tile % a.tiles);
         int64_t first = a.prefix[p.b] + (int64_t)p.h * head_blocks(a, history);
         for (int x = 0; x < t; ++x) first += tile_blocks(a, history, x);
         const int64_t c0 = first / chunk, c1 = (first + tile_blocks(a, history, t) - 1) / chunk;
-        float m = -INFINITY, l = 0.f;
         const int64_t piece0 = (p.tile + c0) * a.rows + p.in;
         const int n = (int)(c1 - c0) + 1;
         const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + piece0;
-#pragma unroll 8
-        for (int c = 0; c < n; ++c) m = fmaxf(m, ml[(int64_t)c * a.rows].x);
+#pragma unroll 4
+        for (int c = group; c < n; c += groups) m = fmaxf(m, ml[(int64_t)c * a.rows].x);
 #pragma unroll 2
-        for (int c = 0; c < n; ++c) {
+        for (int c = group; c < n; c += groups) {
             const float2 x = ml[(int64_t)c * a.rows];
             const float4 *src = reinterpret_cast<const float4 *>(a.part_o + (piece0 + (int64_t)c * a.rows) * TQ_D + 32 * part);
             const float f = x.y == 0.f ? 0.f : exp2f(x.x - m);  // (a piece in which the row saw nothing)
             l += f * x.y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float4 v = src[i];
+                const float4 v = src[2 * turned(part, i >> 1) + (i & 1)];
                 o[4 * i] += f * v.x, o[4 * i + 1] += f * v.y, o[4 * i + 2] += f * v.z, o[4 * i + 3] += f * v.w;
             }
         }
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] *= inv;
     }
+    if (groups > 1) {
+        if (part == 0) s_ml[slot] = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_part[slot * 33 + 8 * part + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        __syncthreads();
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        if (p.live && group == 0) {
+            m = -INFINITY;
+            for (int x = 0; x < groups; ++x) m = fmaxf(m, s_ml[x * rows + row].x);
+            for (int x = 0; x < groups; ++x) {
+                const float2 ml = s_ml[x * rows + row];
+                const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - m);
+                l += f * ml.y;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float4 v = s_part[(x * rows + row) * 33 + 8 * part + i];
+                    o[4 * i] += f * v.x, o[4 * i + 1] += f * v.y, o[4 * i + 2] += f * v.z, o[4 * i + 3] += f * v.w;
+                }
+            }
+        }
+        p.live = p.live && group == 0;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] *= inv;
     float most = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(o[i]));
-    s_most[part][row] = most;
+    s_most[part][slot] = most;
     __syncthreads();
-    most = fmaxf(fmaxf(s_most[0][row], s_most[1][row]), fmaxf(s_most[2][row], s_most[3][row]));
+    most = fmaxf(fmaxf(s_most[0][slot], s_most[1][slot]), fmaxf(s_most[2][slot], s_most[3][slot]));
     // the power of two from the exponent's bits; what is too small for one is left as it is, and so is infinity
     const int exponent = (int)(__float_as_uint(most) >> 23);
     const int up = exponent == 0 || exponent == 255 ? 0 : min(13 + 127 - exponent, 120);
@@ -730,7 +740,7 @@ template <typename T> cudaError_t launch(const TreeArgs &a, const tq_ctx *ctx, i
         default: return cudaErrorInvalidValue;
     }
     if (e != cudaSuccess) return e;
-    constexpr int smem = kUmmaImageBytes + 1024;
+    constexpr int smem = kUmmaImageBytes + kUmmaRows * 33 * 16 + 1024;
     e = tq_allow_shared<tq_tree_join_kernel<T>>(device, smem);
     return e != cudaSuccess ? e : tq_launch_kernel(tq_tree_join_kernel<T>, dim3(blocks), dim3(kRowThreads), smem, stream, true, a, n_rows, per_cta);
 }
