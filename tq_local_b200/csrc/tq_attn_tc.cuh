@@ -78,6 +78,12 @@ __device__ __forceinline__ void mbar_arrive_one(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 
+// One arrival for a converged warp, after what all of its lanes did before.  (An arrival a lane is 32 operations on one word of shared memory.)
+__device__ __forceinline__ void mbar_arrive_warp(uint32_t bar) {
+    __syncwarp();
+    if (elect_one()) mbar_arrive_one(bar);
+}
+
 template <bool BF16> __device__ __forceinline__ uint32_t pack16(float a, float b) {
     uint32_t r;
     if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(b), "f"(a));

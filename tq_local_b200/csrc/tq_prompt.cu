@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     }
     if (tid == 0) {
-        mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1), mbar_init(bar_ask, 1), mbar_init(bar_clean, 32), mbar_init(bar_clean + 8, 32);
-        for (int i = 0; i < 4; ++i) mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 128);
+        mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1), mbar_init(bar_ask, 1), mbar_init(bar_clean, 1), mbar_init(bar_clean + 8, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 4);
         for (int w = 0; w < 2; ++w) mbar_init(bar_o + 8 * w, 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (row < start - j0 || row >= n_kv - j0) sts128(ring + slot * kSlotBytes + (i & 8) / 8 * kUmmaSlabBytes + row * 128 + (i & 7) * 16, 0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                mbar_arrive_one(bar_clean + (k ? 8 : 0));
+                mbar_arrive_warp(bar_clean + (k ? 8 : 0));
             }
         }
     } else {
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_fence_before();
             // (the wait for the last values tells them from those before only if these are known to be done)
             if (u && u + 1 == mine) wait(bar_o + 8 * w, (u - 1) & 1);
-            mbar_arrive_one(bar_p + 16 * w + 8 * e);
+            mbar_arrive_warp(bar_p + 16 * w + 8 * e);
         }
         // ---------------- the tile's rows
         float l0, l1;

@@ -4,15 +4,21 @@
 //
 //   logit_ij = scale (kn_j c_k[codes_j] . (R_k q_i) + rn_j sqrt(pi/2)/D signs_j . (S q_i)),   out_i = R_v^T sum_j p_ij vn_j c_v[codes_j]
 //
-// Three launches.  The first rotates and projects the queries, rounds them to fp16 (the scale to base 2 and the sketch's factor folded in)
-// and sums up how many blocks of 128 tokens the batch entries have.  The second attends: the 128 rows of a tile are (node, head of the group)
-// pairs, its blocks are those of history and drafted tokens laid end to end, and all tiles' blocks laid end to end are cut into
-// equal pieces, one a CTA (one CTA an SM).  The third joins a tile's pieces, un-rotates and rounds.
+// Three launches.  The first rotates and projects the queries and rounds them to fp16 (the scale to base 2 and the sketch's factor folded in).
+// The second attends: the 128 rows of a tile are (node, head of the group) pairs, its blocks of 128 are those of history and drafted tokens laid
+// end to end, and all tiles' blocks laid end to end are cut into equal pieces, one a CTA (one CTA an SM).  The third joins a tile's pieces,
+// un-rotates and rounds.  The second starts beside the first and turns packed tokens into operands before there are queries.
 //
-// Roles of the second: warps 4-11 turn packed tokens into fp16 operands in shared memory, two threads a token: centres times norm by a
-// table of centre pairs in shared memory, +-rn for the signs.  Warp 12 issues the products, S = [Rq | Sq] [K | signs]^T with the queries in TMEM
-// and O += P V.  Warps 0-3 take the softmax, a row a thread; the weights go back over S as 16-bit pairs.
-// TMEM: S of two blocks, O, the queries, 128 columns each.
+// Roles of the second.  Warps 0-7: softmax, half of a row's tokens a thread; the weights go back over the logits as 16-bit pairs.  Warps 8-23 turn packed
+// tokens into fp16 operands in shared memory: centres times norm by a table of centre pairs, +-rn for the signs; half of them take the even blocks,
+// half the odd ones.  Warp 24 issues the products, S = [Rq | Sq] [K | signs]^T with the queries in TMEM and O += P V.  Warp 25 requests the packed
+// blocks (bulk copies, a ring of three).  TMEM: S of two blocks, O, the queries, 128 columns each.
+//
+// What bounds it: a block of 128 tokens takes a CTA 1.6 to 1.7 us whatever the bits, the sketch and the number of rows.  Of 195 us for 16 nodes over
+// 8 x 32768 tokens (32 / 8 heads, 4 bits, sketch) leaving out the operands' stores gives back 48, the products 28, the look-ups 25, the exponentials 5; with
+// all four left out 109 remain, which is the hand-over from role to role.  Shared memory is three quarters busy (operands written once and read once by the
+// products, which read all of B again for every 128 rows).  Variants measured on the way: operands by eight warps straight from
+// global memory, two stages of everything, 197 us; by sixteen, one block at a time, 247; two stages of values and two of the ring, 227.
 #include <math.h>
 
 #include <type_traits>
@@ -22,7 +28,8 @@
 
 namespace {
 
-constexpr int kSoftmaxWarps = 4, kOperandWarps = 16;  // and four more, of which one issues the products
+constexpr int kRingSlots = 3;
+constexpr int kSoftmaxWarps = 8, kOperandWarps = 16;  // and four more, of which one requests the packed blocks and one issues the products
 constexpr int kThreads = 32 * (kSoftmaxWarps + kOperandWarps + 4);
 constexpr int kBlock = 128;  // tokens of a block
 
@@ -40,7 +47,6 @@ struct TreeArgs {
     const void *q;
     void *out;
     int64_t qb, qh, qt, ob, oh, ot;
-    int64_t *prefix;  // [batch + 1] blocks of the entries before
     uint16_t *qop;    // [batch][kv_heads][tiles][rows][128 or 256] fp16
     float *part_ml, *part_o;  // [piece][rows][2], [piece][rows][128]
     int ctas;
@@ -50,23 +56,58 @@ struct TreeArgs {
 // Where a coordinate lies in the operands and in O: the second and third eight of the last two quarters change places (see the stores below).
 __device__ __forceinline__ int turned(int quarter, int eight) { return eight ^ (quarter & 2); }
 
+// An entry's tokens as the kernel counts them: the cache's tokens from `first` (a multiple of eight, so that every stream can be copied in whole
+// 16 bytes) up to the history's end, places up to the next multiple of eight, then the cache's tokens from tree_start, rounded down to one.
+// The history is [lo, end), node 0 lies at nodes_at.
 struct Entry {
-    int start, history;
+    int first, lo, end, nodes_at;
 };
+__device__ __forceinline__ int up8(int n) { return (n + 7) & ~7; }
 __device__ __forceinline__ Entry entry_of(const TreeArgs &a, int b) {
     const int length = a.lengths ? min(max(a.lengths[b], 0), a.tree_start) : a.tree_start;
     const int start = a.seq_start ? min(max(a.seq_start[b], 0), length) : 0;
-    return {start, length - start};
+    Entry e;
+    e.first = start & ~7, e.lo = start - e.first, e.end = length - e.first, e.nodes_at = up8(e.end) + (a.tree_start & 7);
+    return e;
 }
 // tokens that tile t of an entry may see, in blocks
-__device__ __forceinline__ int tile_blocks(const TreeArgs &a, int history, int t) {
+__device__ __forceinline__ int tile_blocks(const TreeArgs &a, const Entry &e, int t) {
     const int drafted = a.mask ? a.nodes : min(a.nodes, (t + 1) * a.positions);
-    return (history + drafted + kBlock - 1) / kBlock;
+    return (e.nodes_at + drafted + kBlock - 1) / kBlock;
 }
-__device__ __forceinline__ int head_blocks(const TreeArgs &a, int history) {
-    int n = 0;
-    for (int t = 0; t < a.tiles; ++t) n += tile_blocks(a, history, t);
-    return n;
+// How the blocks of all tiles, laid end to end, are cut into pieces of `chunk`, one a CTA.  Where there are no more tiles than CTAs a tile takes whole
+// pieces (`whole`: its length is rounded up to them), if that costs at most two blocks a piece: going from one tile to the next takes a CTA some 5 us,
+// as long as three blocks.
+struct Cut {
+    int64_t total;
+    int chunk;
+    bool whole;
+    __device__ __forceinline__ int length(int blocks) const { return whole ? (blocks + chunk - 1) / chunk * chunk : blocks; }
+};
+__device__ __forceinline__ int64_t entry_length(const TreeArgs &a, const Cut &cut, int b) {  // of all heads' and tiles' blocks
+    const Entry e = entry_of(a, b);
+    int64_t n = 0;
+    for (int t = 0; t < a.tiles; ++t) n += cut.length(tile_blocks(a, e, t));
+    return n * a.kv_heads;
+}
+__device__ __forceinline__ Cut cut_of(const TreeArgs &a, int lane) {  // one warp
+    auto sum = [&](const Cut &cut) {
+        int64_t n = 0;
+        for (int b = lane; b < a.batch; b += 32) n += entry_length(a, cut, b);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        return n;
+    };
+    Cut cut = {0, 1, false};
+    cut.total = sum(cut);
+    cut.chunk = (int)((cut.total + a.ctas - 1) / a.ctas);
+    if ((int64_t)a.batch * a.kv_heads * a.tiles <= a.ctas)
+        for (int c = cut.chunk; c < cut.chunk + 3; ++c) {
+            Cut trial = {0, c, true};
+            trial.total = sum(trial);
+            if (trial.total <= (int64_t)c * a.ctas) return trial;
+        }
+    return cut;
 }
 
 // ---------------------------------------------------------------------------------------------------- 128 x 128 matrices
@@ -90,22 +131,21 @@ __device__ __forceinline__ RowPlace place_of(const TreeArgs &a, int64_t r, int64
     return p;
 }
 
-// TMEM and the barriers of such a kernel, and its product: the rows are in TMEM as hi and lo terms at +256 and +320, the sums come at +128 i.
+// TMEM and the barriers of such a kernel, and its product: the rows are in TMEM as hi and lo terms at +256 and +320, the sums come at +0.
 struct RowTile {
     uint32_t tmem, bar_image, bar_mma;
     bool lost = false;
-    __device__ __forceinline__ void start(uint32_t *s_tmem, uint64_t *s_bars, uint32_t images, const uint16_t *image0, const uint16_t *image1) {
+    __device__ __forceinline__ void start(uint32_t *s_tmem, uint64_t *s_bars, uint32_t at, const uint16_t *image) {
         bar_image = smem_u32(s_bars), bar_mma = bar_image + 8;
         if (threadIdx.x < 32) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)), "r"(512));
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
         }
         if (threadIdx.x == 32) {
-            mbar_init(bar_image, image1 ? 2 : 1), mbar_init(bar_mma, 1);
+            mbar_init(bar_image, 1), mbar_init(bar_mma, 1);
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            umma_load_image(images, image0, bar_image);
-            if (image1) umma_load_image(images + kUmmaImageBytes, image1, bar_image);
+            umma_load_image(at, image, bar_image);
         }
         umma_fence_before();
         __syncthreads();
@@ -125,11 +165,11 @@ struct RowTile {
         umma_fence_before();
         __syncthreads();
     }
-    template <bool TRANSPOSED> __device__ __forceinline__ void multiply(uint32_t images, int n) {
+    template <bool TRANSPOSED> __device__ __forceinline__ void multiply(uint32_t image) {
         if (threadIdx.x < 32 && elect_one()) {
             umma_fence_after();
             if (!mbar_wait(bar_image, 0)) lost = true;
-            for (int i = 0; i < n; ++i) umma_issue<2, TRANSPOSED>(tmem + 128 * i, tmem + 256, tmem + 320, images + i * kUmmaImageBytes);
+            umma_issue<2, TRANSPOSED>(tmem, tmem + 256, tmem + 320, image);
             umma_commit(bar_mma);
         }
         __syncwarp();
@@ -148,32 +188,17 @@ struct RowTile {
     }
 };
 
-// Operand rows [Rq | Sq].  Sketch coordinates lie in the order in which the operand's signs do, (i, i + 16) of 32 side by side.
+// Operand rows [Rq | Sq], blockIdx.y: which.  Sketch coordinates lie in the order in which the operand's signs do, (i, i + 16) of 32 side by side.
 template <typename T, bool QJL> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_prep_kernel(const __grid_constant__ TreeArgs a, int64_t n_rows, int per_cta) {
     constexpr int kWide = QJL ? 256 : 128;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t s_bars[2];
     __shared__ uint32_t s_tmem;
-    const uint32_t images = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t image = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const bool sketch = QJL && blockIdx.y;
     tq_launch_dependents();
     RowTile tile;
-    tile.start(&s_tmem, s_bars, images, a.image_k, QJL ? a.image_s : nullptr);
-    if (blockIdx.x == 0 && threadIdx.x >= kRowThreads - 32) {  // (rows of the last warp are few, or there are many other blocks)
-        const int lane = threadIdx.x & 31;
-        int64_t before = 0;
-        for (int b0 = 0; b0 < a.batch; b0 += 32) {
-            const int b = b0 + lane;
-            int64_t n = b < a.batch ? (int64_t)head_blocks(a, entry_of(a, b).history) * a.kv_heads : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t x = __shfl_up_sync(0xffffffffu, n, o);
-                if (lane >= o) n += x;
-            }
-            if (b < a.batch) a.prefix[b + 1] = before + n;
-            before += __shfl_sync(0xffffffffu, n, 31);
-        }
-        if (lane == 0) a.prefix[0] = 0;
-    }
+    tile.start(&s_tmem, s_bars, image, sketch ? a.image_s : a.image_k);
     const int row = threadIdx.x & 127, part = threadIdx.x >> 7;
     const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
     const int64_t r = (int64_t)blockIdx.x * per_cta + row;
@@ -198,35 +223,34 @@ template <typename T, bool QJL> __global__ void __launch_bounds__(kRowThreads, 1
     }
     __syncwarp();
     tile.put(x, part, lanes);
-    tile.multiply<false>(images, QJL ? 2 : 1);
+    tile.multiply<false>(image);
+    const float f = sketch ? a.unscale_s * (1.2533141373155003f / (float)TQ_D) : a.unscale_k;
+    uint32_t y[32], o[16];
+    tmem_ld32(tile.tmem + lanes + 32 * part, y);
+    tmem_ld_wait(y);
 #pragma unroll
-    for (int i = 0; i < (QJL ? 2 : 1); ++i) {
-        const float f = i ? a.unscale_s * (1.2533141373155003f / (float)TQ_D) : a.unscale_k;
-        uint32_t y[32], o[16];
-        __syncwarp();
-        tmem_ld32(tile.tmem + 128 * i + lanes + 32 * part, y);
-        tmem_ld_wait(y);
+    for (int e = 0; e < 16; ++e)
+        o[e] = half2_bits(__uint_as_float(sketch ? y[e] : y[2 * e]) * f, __uint_as_float(sketch ? y[e + 16] : y[2 * e + 1]) * f);
+    if (mine) {
+        uint4 *dst = reinterpret_cast<uint4 *>(a.qop + r * kWide + (sketch ? 128 : 0) + 32 * part);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int lo = i ? e : 2 * e, hi = i ? e + 16 : 2 * e + 1;
-            o[e] = half2_bits(__uint_as_float(y[lo]) * f, __uint_as_float(y[hi]) * f);
-        }
-        if (mine) {
-            uint4 *dst = reinterpret_cast<uint4 *>(a.qop + r * kWide + 128 * i + 32 * part);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dst[turned(part, e)] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
+        for (int e = 0; e < 4; ++e) dst[turned(part, e)] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
     }
     tile.finish(a.error_flag);
 }
 
 // ---------------------------------------------------------------------------------------------------- attention
-// Shared memory: two stages of keys and of values, one of signs, and the tables of centre pairs.  A slot of a table holds its pair once per
-// lane, so that every lane reads its own bank.
+// Shared memory: operands - two stages of keys, one of signs, one of values -, the tables of centre pairs, and a ring of packed blocks.  A slot of a
+// table holds its pair once per lane, so that every lane reads its own bank.
 template <int KB, int VB, bool QJL> struct Layout {
-    static constexpr int kKeys = 0, kValues = 2 * kUmmaTermBytes, kSigns = 4 * kUmmaTermBytes;
+    static constexpr int kKeys = 0, kValues = 2 * kUmmaTermBytes, kSigns = 3 * kUmmaTermBytes;
     static constexpr int kKeyTable = kSigns + (QJL ? kUmmaTermBytes : 0), kValueTable = kKeyTable + 128 * (1 << 2 * KB);
-    static constexpr int kBytes = kValueTable + 128 * (1 << 2 * VB) + 1024;
+    static constexpr int kRing = kValueTable + 128 * (1 << 2 * VB);
+    // of a slot: the six streams
+    static constexpr int kRawK = 0, kRawV = kRawK + kBlock * 16 * KB, kRawS = kRawV + kBlock * 16 * VB, kRawKN = kRawS + (QJL ? kBlock * 16 : 0),
+                         kRawVN = kRawKN + 2 * kBlock, kRawRN = kRawVN + 2 * kBlock, kSlot = kRawRN + (QJL ? 2 * kBlock : 0);
+    static constexpr int kTokenBytes = kSlot / kBlock;
+    static constexpr int kBytes = kRing + kRingSlots * kSlot + 1024;
 };
 
 // Word i of the operand from 32 codes in BITS words (and one that is not looked at): two neighbouring codes by one look-up, times the norm.
@@ -242,41 +266,43 @@ template <int BITS> __device__ __forceinline__ uint32_t centre_pair(const uint32
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
-// Bits [base, base + 32) of what a row sees, base relative to the first drafted token: all of the history, then the mask.
-__device__ __forceinline__ uint32_t seen_word(uint64_t mask, int chain_end, int base) {
-    uint32_t r = 0;
-    if (base < 0) r = base <= -32 ? 0xffffffffu : (1u << -base) - 1u;
-    if (chain_end >= 0) {  // a chain: nodes [0, chain_end)
-        const int n = chain_end - base;
-        return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : r | ((1u << n) - 1u);
-    }
-    if (base <= -32 || base >= 64) return r;
-    return r | (uint32_t)(base < 0 ? mask << -base : mask >> base);
+// Bits [0, n) of a word, for any n.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+// What a row sees of the 32 tokens from `at`: the history, then its nodes - mask, or as a chain the nodes [0, chain_end).
+__device__ __forceinline__ uint32_t seen_word(const Entry &e, uint64_t mask, int chain_end, int at) {
+    const uint32_t history = low_bits(e.end - at) & ~low_bits(e.lo - at);
+    const int node = at - e.nodes_at;
+    if (chain_end >= 0) return history | (low_bits(chain_end - node) & ~low_bits(-node));
+    if (node <= -32 || node >= 64) return history;
+    return history | (uint32_t)(node < 0 ? mask << -node : mask >> node);
 }
 
 template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 1) tq_tree_kernel(const __grid_constant__ TreeArgs a) {
     using L = Layout<KB, VB, QJL>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 2 + 1 + 1];
+    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 1 + 1 + 1 + 2 + 2 * kRingSlots];
     __shared__ uint32_t s_tmem;
+    __shared__ float s_half[2][kUmmaRows];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = smem_u32(s_bars);
-    // full: operands are there; kfree, vfree: the products that read keys and signs, or values, are done; s: logits are there; p: weights are there;
-    // o: O += P V is done; q: queries are there
-    const uint32_t bar_full = bars, bar_kfree = bars + 16, bar_vfree = bars + 32, bar_s = bars + 48, bar_p = bars + 64, bar_o = bars + 80, bar_q = bars + 88;
+    // kfull, vfull: operands are there; kfree, vfree: the products that read keys and signs, or values, are done; s: logits are there; p: weights are there; o: O += P V is
+    // done; q: queries are there; raw, read: a slot of the ring is filled, has been read
+    const uint32_t bar_kfull = bars, bar_kfree = bars + 16, bar_s = bars + 32, bar_p = bars + 48, bar_o = bars + 64, bar_q = bars + 72, bar_vfull = bars + 80, bar_vfree = bars + 88,
+                   bar_raw = bars + 104, bar_read = bar_raw + 8 * kRingSlots;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int kProducts = kSoftmaxWarps + kOperandWarps;
-    const int row_warps = (a.rows + 31) >> 5;  // warps of the softmax that have rows (the others' rows of S and O are what they are)
+    const int row_warps = (a.rows + 31) >> 5;  // quarters of the tile that have rows (the others' rows of S and O are what they are)
     if (warp == kProducts) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_full + 8 * i, 16 * kOperandWarps), mbar_init(bar_kfree + 8 * i, 1), mbar_init(bar_vfree + 8 * i, 1);
-            mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 32 * row_warps);
+            mbar_init(bar_kfull + 8 * i, kOperandWarps / 2), mbar_init(bar_kfree + 8 * i, 1), mbar_init(bar_vfree + 8 * i, 1);
+            mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 2 * row_warps);
         }
-        mbar_init(bar_o, 1), mbar_init(bar_q, 32 * row_warps);
+        mbar_init(bar_o, 1), mbar_init(bar_q, 2 * row_warps), mbar_init(bar_vfull, kOperandWarps / 2);
+        for (int i = 0; i < kRingSlots; ++i) mbar_init(bar_raw + 8 * i, 1), mbar_init(bar_read + 8 * i, kOperandWarps / 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     {
@@ -290,43 +316,59 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         fill(base + L::kKeyTable, KB, ck);
         fill(base + L::kValueTable, VB, cv);
     }
+    // ---- this CTA's blocks: [flat, flat_end) of all tiles' blocks laid end to end.  (Counted here as well: packed tokens do not wait for the queries.)
+    __shared__ Cut s_cut;
+    __shared__ int64_t s_first;
+    __shared__ int s_entry;
+    if (warp == 0) {
+        const Cut cut = cut_of(a, lane);
+        const int64_t from = (int64_t)blockIdx.x * cut.chunk;
+        int64_t before = 0;
+        for (int b0 = 0; from < cut.total && b0 < a.batch; b0 += 32) {  // the entry that holds block `from`
+            const int64_t mine = b0 + lane < a.batch ? entry_length(a, cut, b0 + lane) : 0;
+            int64_t end = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t x = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end += x;
+            }
+            const bool here = before + end - mine <= from && from < before + end;
+            if (here) s_entry = b0 + lane, s_first = before + end - mine;
+            before += __shfl_sync(0xffffffffu, end, 31);
+            if (__any_sync(0xffffffffu, here)) break;
+        }
+        if (lane == 0) s_cut = cut;
+    }
     umma_fence_before();
     __syncthreads();
     umma_fence_after();
-    tq_grid_dependency_wait();
     tq_launch_dependents();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), t_o = tmem + 256, t_q = tmem + 384;
-
-    // ---- this CTA's blocks: [flat, flat_end) of all tiles' blocks laid end to end
-    const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
-    int64_t flat = (int64_t)blockIdx.x * chunk;
-    const int64_t flat_end = min(flat + chunk, total);
+    const Cut cut = s_cut;
+    int64_t flat = (int64_t)blockIdx.x * cut.chunk;
+    const int64_t flat_end = min(flat + cut.chunk, cut.total);
+    int b_at = 0;
+    int64_t b_first = 0, b_next = 0;
+    if (flat < flat_end) b_at = s_entry, b_first = s_first, b_next = b_first + entry_length(a, cut, b_at);
     struct Segment {  // the part of one tile inside this CTA's piece: blocks [k, k_end)
-        int b, h, t, history, start, k, k_end;
+        int b, h, t, k, k_end;
+        Entry e;
         int64_t tile;
     };
-    int b_at = 0;  // the entry that holds block `flat`
-    if (flat < flat_end)
-        for (int b0 = 0, n = 32; n == 32; b0 += 32) {
-            const int64_t end = a.prefix[min(b0 + lane + 1, a.batch)];
-            n = __popc(__ballot_sync(0xffffffffu, b0 + lane < a.batch && end <= flat));
-            b_at += n;
-        }
-    int64_t b_first = flat < flat_end ? a.prefix[b_at] : 0, b_next = flat < flat_end ? a.prefix[b_at + 1] : 0;
     auto next_segment = [&]() {
-        while (flat >= b_next) ++b_at, b_first = b_next, b_next = a.prefix[b_at + 1];
+        while (flat >= b_next) ++b_at, b_first = b_next, b_next += entry_length(a, cut, b_at);
         Segment g;
-        const Entry e = entry_of(a, b_at);
-        const int per_head = head_blocks(a, e.history);
+        g.e = entry_of(a, b_at), g.b = b_at;
+        const int per_head = (int)((b_next - b_first) / a.kv_heads);
         int in = (int)(flat - b_first);
-        g.b = b_at, g.h = in / per_head, in -= g.h * per_head, g.start = e.start, g.history = e.history;
-        int nb = tile_blocks(a, e.history, 0);
-        for (g.t = 0; in >= nb;) in -= nb, ++g.t, nb = tile_blocks(a, e.history, g.t);
-        g.k = in;
+        g.h = in / per_head, in -= g.h * per_head;
+        int nb = tile_blocks(a, g.e, 0);
+        for (g.t = 0; in >= cut.length(nb);) in -= cut.length(nb), ++g.t, nb = tile_blocks(a, g.e, g.t);
         const int64_t left = flat_end - flat;
-        g.k_end = left < nb - in ? in + (int)left : nb;
+        const int end = left < cut.length(nb) - in ? in + (int)left : cut.length(nb);
+        flat += end - in;
+        g.k = in, g.k_end = min(end, nb);
         g.tile = ((int64_t)g.b * a.kv_heads + g.h) * a.tiles + g.t;
-        flat += g.k_end - g.k;
         return g;
     };
     bool lost = false;  // a wait of this thread ran out: it waits for nothing more
@@ -336,139 +378,179 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
 
     if (warp >= kProducts) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
-        if (warp == kProducts && elect_one()) {
+        if (warp == kProducts) {
             // ---------------- products, by one thread; n counts blocks since the kernel began
-            constexpr uint32_t instr_s = umma_instr<false>(), instr_o = umma_instr<true>();
-            auto scores = [&](uint32_t n) {
-                wait(bar_full + 8 * (n & 1), n >> 1 & 1);
-                umma_fence_after();
-#pragma unroll
-                for (int part = 0; part < (QJL ? 2 : 1); ++part) {
-                    const uint64_t desc = umma_desc<false>(base + (part ? L::kSigns : L::kKeys + (n & 1) * kUmmaTermBytes));
-#pragma unroll
-                    for (uint32_t s = 0; s < 8; ++s)
-                        umma_f16(tmem + 128 * (n & 1), t_q + 64 * part + 8 * s, desc + (((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4), instr_s, part | (s > 0));
-                }
-                umma_commit(bar_s + 8 * (n & 1));
-                umma_commit(bar_kfree + 8 * (n & 1));
-            };
-            uint32_t n = 0, segment = 0;
-            while (flat < flat_end) {
-                const Segment g = next_segment();
-                const uint32_t end = n + (g.k_end - g.k);
-                wait(bar_q, segment++ & 1);
-                scores(n);
-                for (bool first = true; n < end; ++n, first = false) {
-                    if (n + 1 < end) scores(n + 1);
-                    wait(bar_p + 8 * (n & 1), n >> 1 & 1);
+            if (elect_one()) {
+                constexpr uint32_t instr_s = umma_instr<false>(), instr_o = umma_instr<true>();
+                auto scores = [&](uint32_t n) {
+                    wait(bar_kfull + 8 * (n & 1), n >> 1 & 1);
                     umma_fence_after();
-                    attn_values(t_o, tmem + 128 * (n & 1), base + L::kValues + (n & 1) * kUmmaTermBytes, instr_o, !first);
-                    umma_commit(bar_vfree + 8 * (n & 1));
-                    umma_commit(bar_o);
+#pragma unroll
+                    for (int part = 0; part < (QJL ? 2 : 1); ++part) {
+                        const uint64_t desc = umma_desc<false>(base + (part ? L::kSigns : L::kKeys + (n & 1) * kUmmaTermBytes));
+#pragma unroll
+                        for (uint32_t s = 0; s < 8; ++s)
+                            umma_f16(tmem + 128 * (n & 1), t_q + 64 * part + 8 * s, desc + (((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4), instr_s, part | (s > 0));
+                    }
+                    umma_commit(bar_s + 8 * (n & 1));
+                    umma_commit(bar_kfree + 8 * (n & 1));
+                };
+                uint32_t n = 0, segment = 0;
+                while (flat < flat_end) {
+                    const Segment g = next_segment();
+                    const uint32_t end = n + (g.k_end - g.k);
+                    wait(bar_q, segment++ & 1);
+                    scores(n);
+                    for (bool first = true; n < end; ++n, first = false) {
+                        if (n + 1 < end) scores(n + 1);
+                        wait(bar_vfull, n & 1);
+                        wait(bar_p + 8 * (n & 1), n >> 1 & 1);
+                        umma_fence_after();
+                        attn_values(t_o, tmem + 128 * (n & 1), base + L::kValues, instr_o, !first);
+                        umma_commit(bar_vfree + 8 * (n & 1));
+                        umma_commit(bar_o);
+                    }
+                }
+            }
+        } else if (warp == kProducts + 1) {
+            // ---------------- packed blocks: bulk copies of whole eights of tokens, kRingSlots blocks ahead
+            if (elect_one()) {
+                uint32_t n = 0;
+                while (flat < flat_end) {
+                    const Segment g = next_segment();
+                    const int64_t row = g.b * a.cache_sb + g.h * a.cache_sh;
+                    const int tree = up8(g.e.end), tree_end = tree + up8((a.tree_start & 7) + a.nodes);  // places of the second run of tokens
+                    for (int k = g.k; k < g.k_end; ++k, ++n) {
+                        const int slot = n % kRingSlots, at = k * kBlock;
+                        if (n >= kRingSlots) wait(bar_read + 8 * slot, (n / kRingSlots & 1) ^ 1);
+                        const uint32_t bar = bar_raw + 8 * slot, dst = base + L::kRing + slot * L::kSlot;
+                        const int n0 = max(min(kBlock, tree - at), 0), n1 = max(min(kBlock, tree_end - at) - n0, 0);
+                        mbar_expect_tx(bar, (n0 + n1) * L::kTokenBytes);
+                        auto run = [&](int to, int64_t t, int count) {
+                            tma_load_1d(dst + L::kRawK + to * 16 * KB, a.k_codes + t * 16 * KB, count * 16 * KB, bar);
+                            tma_load_1d(dst + L::kRawV + to * 16 * VB, a.v_codes + t * 16 * VB, count * 16 * VB, bar);
+                            tma_load_1d(dst + L::kRawKN + to * 2, a.k_norms + t, count * 2, bar);
+                            tma_load_1d(dst + L::kRawVN + to * 2, a.v_norms + t, count * 2, bar);
+                            if (QJL) {
+                                tma_load_1d(dst + L::kRawS + to * 16, a.k_signs + t * 16, count * 16, bar);
+                                tma_load_1d(dst + L::kRawRN + to * 2, a.k_rnorms + t, count * 2, bar);
+                            }
+                        };
+                        if (n0) run(0, row + g.e.first + at, n0);
+                        if (n1) run(n0, row + (a.tree_start & ~7) + at + n0 - tree, n1);
+                    }
                 }
             }
         }
     } else if (warp >= kSoftmaxWarps) {
-        // ---------------- operands.  Half of the warps take the even blocks, half the odd ones: a thread's loads have two blocks' time to arrive, and
-        // none are on their way when it fences its stores (the fence would wait for them).  A quarter of two tokens' coordinates a thread, four
-        // lanes to a token, so that a load covers whole lines.
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+        // ---------------- operands.  Half of the warps take the even blocks, half the odd ones, so that one half's waits pass behind the other's
+        // work.  A quarter of two tokens' coordinates a thread, four lanes to a token.
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         const uint32_t half = (uint32_t)(warp - kSoftmaxWarps) / (kOperandWarps / 2);
         const int quarter = lane & 3, row0 = 16 * ((warp - kSoftmaxWarps) % (kOperandWarps / 2)) + (lane >> 2);  // and row0 + 8
-        uint32_t kw[2][KB + 1] = {}, vw[2][VB + 1] = {}, sw[2] = {};
-        uint16_t kn[2], vn[2], rn[2];
-        Segment g;
-        int k = 0, k_end = 0;
-        uint32_t n = 0;  // blocks since the kernel began
-        auto words = [&](const uint8_t *src, auto count, uint32_t *w) {
-            constexpr int n = decltype(count)::value;
-            if constexpr (n == 4) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(src));
-                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-            } else if constexpr (n == 2) {
-                const uint2 x = __ldg(reinterpret_cast<const uint2 *>(src));
-                w[0] = x.x, w[1] = x.y;
-            } else {
-#pragma unroll
-                for (int i = 0; i < n; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
-            }
-        };
-        auto next_block = [&]() {  // false behind the last
-            if (k == k_end) {
-                if (flat >= flat_end) return false;
-                g = next_segment(), k = g.k, k_end = g.k_end;
-            }
-            return true;
-        };
-        auto fetch = [&]() {  // the block's tokens of this thread
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int v = k * kBlock + row0 + 8 * i;
-                kn[i] = vn[i] = rn[i] = 0;
-                if (v < g.history + a.nodes) {
-                    const int64_t t = g.b * a.cache_sb + g.h * a.cache_sh + (v < g.history ? g.start + v : a.tree_start + v - g.history);
-                    words(a.k_codes + t * 16 * KB + 4 * KB * quarter, std::integral_constant<int, KB>(), kw[i]);
-                    words(a.v_codes + t * 16 * VB + 4 * VB * quarter, std::integral_constant<int, VB>(), vw[i]);
-                    kn[i] = __ldg(a.k_norms + t), vn[i] = __ldg(a.v_norms + t);
-                    if (QJL) sw[i] = __ldg(reinterpret_cast<const uint32_t *>(a.k_signs + t * 16) + quarter), rn[i] = __ldg(a.k_rnorms + t);
-                }
-            }
-        };
         const uint32_t lane_k = base + L::kKeyTable + 4 * lane, lane_v = base + L::kValueTable + 4 * lane;
         // Eight lanes store two tokens' quarters: with the last two quarters' eights turned, to eight different banks of 16 bytes.
-        const uint32_t turn = (quarter & 1) * 4 ^ (quarter & 2) ^ (row0 & 7), stage = half * kUmmaTermBytes;
+        const uint32_t turn = (quarter & 1) * 4 ^ (quarter & 2) ^ (row0 & 7);
         const uint32_t my_row = base + (quarter >> 1) * kUmmaSlabBytes + (row0 >> 3) * 1024 + (row0 & 7) * 128;
-        auto put = [&](uint32_t at, auto word) {  // word(i, j): word j of the 16 of token i
+        auto put = [&](uint32_t at, auto word) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    sts128(my_row + at + 1024 * i + ((c ^ turn) << 4), word(i, 4 * c), word(i, 4 * c + 1), word(i, 4 * c + 2), word(i, 4 * c + 3));
+            for (int c = 0; c < 4; ++c) sts128(my_row + at + ((c ^ turn) << 4), word(4 * c), word(4 * c + 1), word(4 * c + 2), word(4 * c + 3));
         };
-        for (; next_block(); ++n, ++k) {
-            if ((n & 1) != half) continue;
-            fetch();
-            if (n > 1) wait(bar_vfree + 8 * half, (n >> 1 & 1) ^ 1);  // (two blocks ago; its logits came before)
-            put(L::kKeys + stage, [&](int i, int j) { return centre_pair<KB>(kw[i], j, lane_k, kn[i] * 0x10001u); });
-            put(L::kValues + stage, [&](int i, int j) { return centre_pair<VB>(vw[i], j, lane_v, vn[i] * 0x10001u); });
-            if (QJL) {
-                if (n) wait(bar_kfree + 8 * (half ^ 1), (n - 1) >> 1 & 1);  // (the signs have one stage)
-                put(L::kSigns, [&](int i, int j) {  // signs j and j + 16 of a word; a set bit is +
-                    return ((sw[i] << (15 - j)) & 0x80008000u) ^ (rn[i] * 0x10001u) ^ 0x80008000u;
-                });
+        auto words = [&](uint32_t src, auto count, uint32_t *w) {
+            constexpr int n = decltype(count)::value;
+            if constexpr (n == 4) {
+                const uint4 x = lds128(src);
+                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < n; ++i) asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[i]) : "r"(src + 4 * i) : "memory");
             }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            mbar_arrive_one(bar_full + 8 * half);
+            w[n] = 0;
+        };
+        auto norm2 = [&](uint32_t src, bool token) {  // (what is no token holds anything)
+            uint16_t x;
+            asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(x) : "r"(src) : "memory");
+            return token ? x * 0x10001u : 0u;
+        };
+        uint32_t n = 0;
+        while (flat < flat_end) {
+            const Segment g = next_segment();
+            for (int k = g.k; k < g.k_end; ++k, ++n) {
+                if ((n & 1) != half) continue;
+                const int slot = n % kRingSlots;
+                const uint32_t raw = base + L::kRing + slot * L::kSlot, stage = L::kKeys + half * kUmmaTermBytes;
+                auto token = [&](int i) {
+                    const int v = k * kBlock + row0 + 8 * i;
+                    return (v >= g.e.lo && v < g.e.end) || (v >= g.e.nodes_at && v < g.e.nodes_at + a.nodes);
+                };
+                wait(bar_raw + 8 * slot, n / kRingSlots & 1);
+                if (n > 1) wait(bar_kfree + 8 * half, (n >> 1 & 1) ^ 1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int row = row0 + 8 * i;
+                    uint32_t w[KB + 1];
+                    words(raw + L::kRawK + row * 16 * KB + 4 * KB * quarter, std::integral_constant<int, KB>(), w);
+                    const uint32_t norm = norm2(raw + L::kRawKN + 2 * row, token(i));
+                    put(stage + 1024 * i, [&](int j) { return centre_pair<KB>(w, j, lane_k, norm); });
+                }
+                if (QJL) {
+                    if (n) wait(bar_kfree + 8 * (half ^ 1), (n - 1) >> 1 & 1);  // (the signs have one stage)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = row0 + 8 * i;
+                        uint32_t w[2];
+                        words(raw + L::kRawS + row * 16 + 4 * quarter, std::integral_constant<int, 1>(), w);
+                        const uint32_t norm = norm2(raw + L::kRawRN + 2 * row, token(i)) ^ 0x80008000u;
+                        put(L::kSigns + 1024 * i, [&](int j) { return ((w[0] << (15 - j)) & 0x80008000u) ^ norm; });  // signs j and j + 16; a set bit is +
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                mbar_arrive_warp(bar_kfull + 8 * half);
+                uint32_t vw[2][VB + 1], vn2[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int row = row0 + 8 * i;
+                    words(raw + L::kRawV + row * 16 * VB + 4 * VB * quarter, std::integral_constant<int, VB>(), vw[i]);
+                    vn2[i] = norm2(raw + L::kRawVN + 2 * row, token(i));
+                }
+                mbar_arrive_warp(bar_read + 8 * slot);
+                if (n) wait(bar_vfree + 8 * (half ^ 1), (n - 1) >> 1 & 1);  // (the values have one stage)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) put(L::kValues + 1024 * i, [&](int j) { return centre_pair<VB>(vw[i], j, lane_v, vn2[i]); });
+                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                mbar_arrive_warp(bar_vfull);
+            }
         }
     } else {
-        // ---------------- softmax, one row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
-        const int row = tid;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        // ---------------- softmax: half of a row's tokens, and of its output's coordinates, a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n");
+        const int half = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, t_mine = t_o + lanes + 64 * half;
         constexpr int kWide = QJL ? 256 : 128;
+        // the two warps that share 32 rows
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + (warp & 3)) : "memory"); };
         uint32_t n = 0;
-        if (warp < row_warps) while (flat < flat_end) {
+        tq_grid_dependency_wait();  // (the queries)
+        if ((warp & 3) < row_warps) while (flat < flat_end) {
             const Segment g = next_segment();
             const int node = g.t * a.positions + row / a.group;
             const bool live = row < a.rows && node < a.nodes;
             const uint64_t mask = live && a.mask ? a.mask[(int64_t)g.b * a.nodes + node] & (~0ull >> (64 - a.nodes)) : 0;
             const int chain_end = a.mask ? -1 : live ? node + 1 : 0;
             // ---- the queries (the products that read the ones before are done: their logits were here)
-            const uint4 *src = reinterpret_cast<const uint4 *>(a.qop + (g.tile * a.rows + row) * kWide);
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.qop + (g.tile * a.rows + row) * kWide) + kWide / 16 * half;
+            uint32_t q[kWide / 4];
 #pragma unroll
-            for (int i = 0; i < kWide / 64; ++i) {
-                uint32_t r[32];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint4 x = row < a.rows ? src[8 * i + e] : make_uint4(0, 0, 0, 0);
-                    r[4 * e] = x.x, r[4 * e + 1] = x.y, r[4 * e + 2] = x.z, r[4 * e + 3] = x.w;
-                }
-                __syncwarp();
-                tmem_st32(t_q + lanes + 32 * i, r);
+            for (int e = 0; e < kWide / 16; ++e) {
+                const uint4 x = row < a.rows ? src[e] : make_uint4(0, 0, 0, 0);
+                q[4 * e] = x.x, q[4 * e + 1] = x.y, q[4 * e + 2] = x.z, q[4 * e + 3] = x.w;
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kWide / 128; ++i) tmem_st32(t_q + lanes + kWide / 4 * half + 32 * i, q + 32 * i);
             tmem_st_wait();
             umma_fence_before();
-            mbar_arrive_one(bar_q);
+            mbar_arrive_warp(bar_q);
             float m_ref = -INFINITY;
             uint64_t sum[2] = {0, 0};
             for (int k = g.k; k < g.k_end; ++k, ++n) {
@@ -476,15 +558,13 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                 wait(bar_s + 8 * (n & 1), n >> 1 & 1);
                 __syncwarp();
                 umma_fence_after();
-                uint32_t s[128];
+                uint32_t s[64];
+                tmem_ld32(t_s + 64 * half, s), tmem_ld32(t_s + 64 * half + 32, s + 32);
+                tmem_ld_wait(s), tmem_ld_wait(s + 32);
+                if ((k + 1) * kBlock > g.e.end || k * kBlock < g.e.lo) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32(t_s + 32 * i, s + 32 * i);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld_wait(s + 32 * i);
-                if ((k + 1) * kBlock > g.history) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const uint32_t seen = seen_word(mask, chain_end, k * kBlock + 32 * x - g.history);
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t seen = seen_word(g.e, mask, chain_end, k * kBlock + 64 * half + 32 * x);
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (!(seen >> i & 1)) s[32 * x + i] = 0xff800000u;
@@ -494,11 +574,16 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top[i] = max3(__uint_as_float(s[i]), __uint_as_float(s[i + 4]), __uint_as_float(s[i + 8]));
 #pragma unroll
-                for (int i = 12; i < 124; i += 8)
+                for (int i = 12; i < 60; i += 8)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
-                float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                peak = fmaxf(peak, max3(__uint_as_float(s[124]), __uint_as_float(s[125]), fmaxf(__uint_as_float(s[126]), __uint_as_float(s[127]))));
+                const float last = max3(__uint_as_float(s[60]), __uint_as_float(s[61]), fmaxf(__uint_as_float(s[62]), __uint_as_float(s[63])));
+                float peak = max3(max3(top[0], top[1], top[2]), top[3], last);
+                s_half[half][row] = peak;
+                umma_fence_before();
+                pair_sync();  // (both have read their logits as well: the weights go over them)
+                umma_fence_after();
+                peak = fmaxf(peak, s_half[half ^ 1][row]);
                 if (k == g.k) {
                     m_ref = peak;
                 } else {
@@ -513,55 +598,59 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                         umma_fence_after();
 #pragma unroll 1
                         for (int i = 0; i < 4; ++i) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + lanes + 32 * i, o);
-                            tmem_ld_wait(o);
+                            uint32_t o[16];
+                            tmem_ld16(t_mine + 16 * i, o);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_st32(t_o + lanes + 32 * i, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st16(t_mine + 16 * i, o);
                         }
                     }
                 }
                 const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
                 const uint64_t shift2 = f32x2(shift, shift);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t p[32];
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         float x, y;
-                        f32x2_split(f32x2_add(f32x2(__uint_as_float(s[64 * half + 2 * i]), __uint_as_float(s[64 * half + 2 * i + 1])), shift2), x, y);
+                        f32x2_split(f32x2_add(f32x2(__uint_as_float(s[32 * part + 2 * i]), __uint_as_float(s[32 * part + 2 * i + 1])), shift2), x, y);
                         x = exp2_hw(x), y = exp2_hw(y);
                         sum[i & 1] = f32x2_add(sum[i & 1], f32x2(x, y));
                         p[i] = pack16<false>(x, y);
                     }
-                    tmem_st32(t_s + 32 * half, p);
+                    tmem_st16(t_s + 32 * half + 16 * part, p);
                 }
                 tmem_st_wait();
                 umma_fence_before();
                 // (the wait for the last values tells them from those before only if these are known to be done)
                 if (k > g.k && k + 1 == g.k_end) wait(bar_o, (n - 1) & 1);
-                mbar_arrive_one(bar_p + 8 * (n & 1));
+                mbar_arrive_warp(bar_p + 8 * (n & 1));
             }
             // ---- this piece of the tile's rows
             float l0, l1;
             f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
+            pair_sync();  // (the last peak has been read)
+            s_half[half][row] = l0 + l1;
+            pair_sync();
+            const float l = s_half[0][row] + s_half[1][row];
             wait(bar_o, (n - 1) & 1);
             __syncwarp();
             umma_fence_after();
             const int64_t r = (g.tile + blockIdx.x) * a.rows + row;
-            if (live) *reinterpret_cast<float2 *>(a.part_ml + 2 * r) = make_float2(m_ref, l0 + l1);
+            if (live && half == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * r) = make_float2(m_ref, l);
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 uint32_t o[32];
                 __syncwarp();
-                tmem_ld32(t_o + lanes + 32 * i, o);
+                tmem_ld32(t_mine + 32 * i, o);
                 tmem_ld_wait(o);
                 if (live)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(a.part_o + r * TQ_D + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(a.part_o + r * TQ_D + 64 * half + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
             umma_fence_before();
+            pair_sync();  // (the sums have been read)
         }
     }
     if (lost) atomicExch(a.error_flag, 8);
@@ -582,10 +671,12 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
     __shared__ uint32_t s_tmem;
     __shared__ float s_most[4][128];
     __shared__ float2 s_ml[128];
-    const uint32_t images = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    float4 *const s_part = reinterpret_cast<float4 *>(smem_raw + (images - smem_u32(smem_raw)) + kUmmaImageBytes);  // [slot][33]
+    __shared__ Cut s_cut;
+    __shared__ float s_sum[128];
+    const uint32_t image = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    float4 *const s_part = reinterpret_cast<float4 *>(smem_raw + (image - smem_u32(smem_raw)) + kUmmaImageBytes);  // [slot][33]
     RowTile tile;
-    tile.start(&s_tmem, s_bars, images, a.image_v, nullptr);
+    tile.start(&s_tmem, s_bars, image, a.image_v);
     const int slot = threadIdx.x & 127, part = threadIdx.x >> 7;
     const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
     int rows = 8;
@@ -594,30 +685,43 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
     const int64_t r = (int64_t)blockIdx.x * per_cta + row;
     RowPlace p = {};
     if (row < per_cta && r < n_rows) p = place_of(a, r, n_rows);
+    // which pieces a row has: counted again, while the second launch runs
+    if (threadIdx.x < 32) {
+        const Cut cut = cut_of(a, threadIdx.x);
+        if (threadIdx.x == 0) s_cut = cut;
+    }
+    __syncthreads();
+    int64_t piece0 = 0;
+    int n = 0;
+    if (p.live) {
+        const Cut cut = s_cut;
+        const Entry e = entry_of(a, p.b);
+        const int t = (int)(p.tile % a.tiles), nb = tile_blocks(a, e, t);
+        int64_t first = entry_length(a, cut, p.b) / a.kv_heads * p.h;
+        for (int b = 0; b < p.b; ++b) first += entry_length(a, cut, b);
+        for (int x = 0; x < t; ++x) first += cut.length(tile_blocks(a, e, x));
+        const int64_t c0 = first / cut.chunk;
+        piece0 = (p.tile + c0) * a.rows + p.in, n = (int)((first + nb - 1) / cut.chunk - c0) + 1;
+    }
     tq_grid_dependency_wait();
     float o[32] = {};
     float m = -INFINITY, l = 0.f;
     if (p.live) {
-        const int64_t total = a.prefix[a.batch], chunk = (total + a.ctas - 1) / a.ctas;
-        const int history = entry_of(a, p.b).history, t = (int)(p.tile % a.tiles);
-        int64_t first = a.prefix[p.b] + (int64_t)p.h * head_blocks(a, history);
-        for (int x = 0; x < t; ++x) first += tile_blocks(a, history, x);
-        const int64_t c0 = first / chunk, c1 = (first + tile_blocks(a, history, t) - 1) / chunk;
-        const int64_t piece0 = (p.tile + c0) * a.rows + p.in;
-        const int n = (int)(c1 - c0) + 1;
-        const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + piece0;
-#pragma unroll 4
-        for (int c = group; c < n; c += groups) m = fmaxf(m, ml[(int64_t)c * a.rows].x);
 #pragma unroll 2
         for (int c = group; c < n; c += groups) {
-            const float2 x = ml[(int64_t)c * a.rows];
-            const float4 *src = reinterpret_cast<const float4 *>(a.part_o + (piece0 + (int64_t)c * a.rows) * TQ_D + 32 * part);
-            const float f = x.y == 0.f ? 0.f : exp2f(x.x - m);  // (a piece in which the row saw nothing)
-            l += f * x.y;
+            const int64_t piece = piece0 + (int64_t)c * a.rows;
+            const float2 x = reinterpret_cast<const float2 *>(a.part_ml)[piece];
+            const float4 *src = reinterpret_cast<const float4 *>(a.part_o + piece * TQ_D + 32 * part);
+            float4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = src[2 * turned(part, i >> 1) + (i & 1)];
+            if (x.y == 0.f) continue;  // (a piece in which the row saw nothing)
+            const float top = fmaxf(m, x.x), keep = exp2f(m - top), f = exp2f(x.x - top);
+            m = top, l = l * keep + f * x.y;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float4 v = src[2 * turned(part, i >> 1) + (i & 1)];
-                o[4 * i] += f * v.x, o[4 * i + 1] += f * v.y, o[4 * i + 2] += f * v.z, o[4 * i + 3] += f * v.w;
+                o[4 * i] = o[4 * i] * keep + f * v[i].x, o[4 * i + 1] = o[4 * i + 1] * keep + f * v[i].y;
+                o[4 * i + 2] = o[4 * i + 2] * keep + f * v[i].z, o[4 * i + 3] = o[4 * i + 3] * keep + f * v[i].w;
             }
         }
     }
@@ -626,22 +730,27 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
 #pragma unroll
         for (int i = 0; i < 8; ++i) s_part[slot * 33 + 8 * part + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         __syncthreads();
-        l = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        if (p.live && group == 0) {
-            m = -INFINITY;
-            for (int x = 0; x < groups; ++x) m = fmaxf(m, s_ml[x * rows + row].x);
+        for (int i = threadIdx.x; i < rows * 32; i += kRowThreads) {  // four coordinates of a row, from its groups
+            const int r0 = i >> 5, c = i & 31;
+            float top = -INFINITY, sum = 0.f;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int x = 0; x < groups; ++x) top = fmaxf(top, s_ml[x * rows + r0].x);
             for (int x = 0; x < groups; ++x) {
-                const float2 ml = s_ml[x * rows + row];
-                const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - m);
-                l += f * ml.y;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 v = s_part[(x * rows + row) * 33 + 8 * part + i];
-                    o[4 * i] += f * v.x, o[4 * i + 1] += f * v.y, o[4 * i + 2] += f * v.z, o[4 * i + 3] += f * v.w;
-                }
+                const float2 ml = s_ml[x * rows + r0];
+                const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - top);
+                const float4 v = s_part[(x * rows + r0) * 33 + c];
+                sum += f * ml.y;
+                y = make_float4(y.x + f * v.x, y.y + f * v.y, y.z + f * v.z, y.w + f * v.w);
             }
+            s_part[r0 * 33 + c] = y;  // (nobody else reads these of group 0)
+            if (c == 0) s_sum[r0] = sum;
+        }
+        __syncthreads();
+        l = group == 0 ? s_sum[row] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 v = group == 0 ? s_part[row * 33 + 8 * part + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            o[4 * i] = v.x, o[4 * i + 1] = v.y, o[4 * i + 2] = v.z, o[4 * i + 3] = v.w;
         }
         p.live = p.live && group == 0;
     }
@@ -662,7 +771,7 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
     for (int i = 0; i < 32; ++i) o[i] *= raise;
     __syncwarp();
     tile.put(o, part, lanes);
-    tile.multiply<true>(images, 1);
+    tile.multiply<true>(image);
     uint32_t y[32];
     tmem_ld32(tile.tmem + lanes + 32 * part, y);
     tmem_ld_wait(y);
@@ -688,7 +797,7 @@ bool aligned(const tq_dense_desc *d) {
 struct Plan {
     int positions, tiles, rows, ctas;
     int64_t n_tiles;
-    size_t prefix, qop, ml, o, bytes;  // workspace offsets
+    size_t qop, ml, o, bytes;  // workspace offsets
 };
 Plan plan(const tq_ctx *ctx, int64_t batch, int q_heads, int kv_heads, int nodes, int tree_start) {
     Plan p;
@@ -697,15 +806,17 @@ Plan plan(const tq_ctx *ctx, int64_t batch, int q_heads, int kv_heads, int nodes
     p.tiles = (nodes + p.positions - 1) / p.positions;
     p.rows = (nodes < p.positions ? nodes : p.positions) * group;
     p.n_tiles = batch * kv_heads * p.tiles;
-    const int64_t most = p.n_tiles * (((int64_t)tree_start + nodes + kBlock - 1) / kBlock);
-    p.ctas = most < ctx->sm_count ? (int)most : ctx->sm_count;
+    const int64_t most = p.n_tiles * (((int64_t)tree_start + nodes + 21 + kBlock - 1) / kBlock);  // (with the places between, see Entry)
+    // a CTA an SM; where the queries' CTAs are few, the others', which then start beside them
+    const int64_t prep = (p.n_tiles * p.rows + kUmmaRows - 1) / kUmmaRows * (ctx->use_qjl ? 2 : 1);
+    const int sms = prep <= 8 ? ctx->sm_count - (int)prep : ctx->sm_count;
+    p.ctas = most < sms ? (int)most : sms;
     auto take = [at = (size_t)0](size_t bytes) mutable {
         const size_t r = at;
         at += (bytes + 255) / 256 * 256;
         return r;
     };
     const size_t pieces = (size_t)(p.n_tiles + p.ctas) * p.rows;
-    p.prefix = take((batch + 1) * sizeof(int64_t));
     p.qop = take((size_t)p.n_tiles * p.rows * (ctx->use_qjl ? 512 : 256));
     p.ml = take(pieces * 2 * sizeof(float));
     p.o = take(pieces * TQ_D * sizeof(float));
@@ -720,9 +831,9 @@ template <int KB, int VB, bool QJL> cudaError_t launch_attend(const TreeArgs &a,
 }
 
 template <typename T, bool QJL> cudaError_t launch_prep(const TreeArgs &a, int64_t n_rows, unsigned blocks, int per_cta, int device, cudaStream_t stream) {
-    constexpr int smem = (QJL ? 2 : 1) * kUmmaImageBytes + 1024;
+    constexpr int smem = kUmmaImageBytes + 1024;
     const cudaError_t e = tq_allow_shared<tq_tree_prep_kernel<T, QJL>>(device, smem);
-    return e != cudaSuccess ? e : tq_launch_kernel(tq_tree_prep_kernel<T, QJL>, dim3(blocks), dim3(kRowThreads), smem, stream, false, a, n_rows, per_cta);
+    return e != cudaSuccess ? e : tq_launch_kernel(tq_tree_prep_kernel<T, QJL>, dim3(blocks, QJL ? 2 : 1), dim3(kRowThreads), smem, stream, false, a, n_rows, per_cta);
 }
 
 template <typename T> cudaError_t launch(const TreeArgs &a, const tq_ctx *ctx, int64_t n_rows, cudaStream_t stream) {
@@ -731,7 +842,8 @@ template <typename T> cudaError_t launch(const TreeArgs &a, const tq_ctx *ctx, i
     const int64_t share = ((n_rows + ctx->sm_count - 1) / ctx->sm_count + 7) / 8 * 8;
     const int per_cta = share < kUmmaRows ? (int)share : kUmmaRows;
     const unsigned blocks = (unsigned)((n_rows + per_cta - 1) / per_cta);
-    cudaError_t e = qjl ? launch_prep<T, true>(a, n_rows, blocks, per_cta, device, stream) : launch_prep<T, false>(a, n_rows, blocks, per_cta, device, stream);
+    const unsigned prep_blocks = (unsigned)((n_rows + kUmmaRows - 1) / kUmmaRows);  // (few CTAs: the others of the second launch do not wait for their SMs)
+    cudaError_t e = qjl ? launch_prep<T, true>(a, n_rows, prep_blocks, kUmmaRows, device, stream) : launch_prep<T, false>(a, n_rows, prep_blocks, kUmmaRows, device, stream);
     if (e != cudaSuccess) return e;
     switch (ctx->bits) {
         case 2: e = qjl ? launch_attend<1, 2, true>(a, device, stream) : launch_attend<2, 2, false>(a, device, stream); break;
@@ -782,7 +894,7 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v;
     a.q = q->data, a.qb = q->stride_b, a.qh = q->stride_h, a.qt = q->stride_t;
     a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
-    a.prefix = reinterpret_cast<int64_t *>(ws + p.prefix), a.qop = reinterpret_cast<uint16_t *>(ws + p.qop);
+    a.qop = reinterpret_cast<uint16_t *>(ws + p.qop);
     a.part_ml = reinterpret_cast<float *>(ws + p.ml), a.part_o = reinterpret_cast<float *>(ws + p.o);
     a.error_flag = ctx->error_flag;
     TQ_CUDA_CHECK(q->dtype == TQ_DTYPE_F16 ? launch<__half>(a, ctx, n_rows, (cudaStream_t)stream)
