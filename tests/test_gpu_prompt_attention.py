@@ -163,6 +163,20 @@ def test_packed_sequences(hq, hkv, dtype):
     assert torch.equal(prompt_attention_packed(q, k, v, cu, 500)[131:131 + 77], mine)
 
 
+def test_sequence_bounds_outside_the_tensor_are_cut():
+    from tq_local_b200.runtime.prompt_attention import prompt_attention_packed
+
+    q, k, v = (t[0].transpose(0, 1) for t in make(1, 4, 2, 300, 300, BF16, 4))
+    room = torch.full((400, 4, 128), 7.0, dtype=BF16, device="cuda")
+    out = room[:300]
+    cu = torch.tensor([-50, 100, 90, 250, 1000], dtype=torch.int32, device="cuda")  # [0, 100), nothing, [90, 250), [250, 300)
+    prompt_attention_packed(q, k, v, cu, 300, out=out)
+    for lo, hi in ((0, 90), (250, 300)):  # (what two sequences share is either's)
+        part = [t[(0 if lo == 0 else lo):hi].transpose(0, 1).unsqueeze(0) for t in (q, k, v, out)]
+        check(part[3], *reference(*part[:3]))
+    assert (room[300:] == 7.0).all()
+
+
 def test_many_short_sequences():
     from tq_local_b200.runtime.prompt_attention import prompt_attention_packed
 

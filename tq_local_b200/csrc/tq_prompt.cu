@@ -48,7 +48,7 @@ struct PromptArgs {
     void *out;
     int64_t ob, oh, ot;
     int batch, kv_heads, group, positions;  // positions of a tile: 128 / group
-    int n_q, n_kv, n_items, tiles_per_cta, splits;
+    int n_q, n_kv, total, n_items, tiles_per_cta, splits;
     const int *seq_start, *cu_seqlens;
     float scale_log2;  // |scale| log2(e)
     bool causal, negate;
@@ -66,6 +66,12 @@ __device__ __forceinline__ void load_map(uint32_t dst, const CUtensorMap *map, u
                  : "memory");
 }
 
+// Sequence b of a packed call: its first token, and how many there are - inside [0, total) and no more than n_q, whatever cu_seqlens holds.
+__device__ __forceinline__ int2 sequence_of(const PromptArgs &a, int b) {
+    const int first = min(max(a.cu_seqlens[b], 0), a.total);
+    return make_int2(first, min(min(a.cu_seqlens[b + 1], a.total) - first, a.n_q));
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     tq_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -75,7 +81,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int h = blockIdx.x % a.kv_heads, b = blockIdx.x / a.kv_heads % a.batch;
     const int item = a.n_items - 1 - blockIdx.x / (a.kv_heads * a.batch);
     int n_q = a.n_q, n_kv = a.n_kv, t0 = 0;
-    if (a.cu_seqlens) t0 = a.cu_seqlens[b], n_q = n_kv = min(a.cu_seqlens[b + 1] - t0, a.n_q);
+    if (a.cu_seqlens) {
+        const int2 seq = sequence_of(a, b);
+        t0 = seq.x, n_q = n_kv = seq.y;
+    }
     const int first_pos = item * a.tiles_per_cta * a.positions;
     if (first_pos >= n_q) return;
     const int offset = n_kv - n_q;
@@ -376,8 +385,9 @@ template <bool BF16> __global__ void __launch_bounds__(128) tq_prompt_join_kerne
     const int head = (int)(r % heads), pos = (int)(r / heads % a.n_q), b = (int)(r / heads / a.n_q);
     int t0 = 0;
     if (a.cu_seqlens) {
-        t0 = a.cu_seqlens[b];
-        if (pos >= min(a.cu_seqlens[b + 1] - t0, a.n_q)) return;
+        const int2 seq = sequence_of(a, b);
+        t0 = seq.x;
+        if (pos >= seq.y) return;
     }
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + r * a.splits;
     float m = -INFINITY;
@@ -505,7 +515,7 @@ int32_t prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_den
     PromptArgs a = {};
     a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
     a.batch = batch, a.kv_heads = kv_heads, a.group = q_heads / kv_heads, a.positions = p.positions;
-    a.n_q = n_q, a.n_kv = n_kv, a.n_items = p.n_items, a.tiles_per_cta = p.tiles_per_cta, a.splits = p.splits;
+    a.n_q = n_q, a.n_kv = n_kv, a.total = total, a.n_items = p.n_items, a.tiles_per_cta = p.tiles_per_cta, a.splits = p.splits;
     a.seq_start = seq_start, a.cu_seqlens = cu_seqlens, a.causal = causal != 0, a.negate = scale < 0.f;
     a.scale_log2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);  // (not 0: a masked logit is -inf and has to stay so)
     if (p.splits > 1) {
