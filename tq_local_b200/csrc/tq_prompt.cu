@@ -344,9 +344,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else {
-            uint8_t *dst = reinterpret_cast<uint8_t *>(a.out) + 2 * ((a.cu_seqlens ? 0 : b) * a.ob + head * a.oh + (int64_t)(t0 + pos) * a.ot);
+            // Rows leave through the tile's query image, which nobody reads any more, sixteen lanes to a row: a warp's 32 rows of 256 bytes, 16-byte
+            // pieces turned by the row.
             const bool any = l > 0.f || l != l;
             const float inv = any ? 1.f / l : 0.f;
+            const int lane = tid & 31;
+            const uint32_t stage = base + w * kSlotBytes + (warp & 3) * 32 * 256, turn = lane & 15;
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 uint32_t o[32] = {};
@@ -355,16 +358,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(t_o + 32 * i, o);
                     tmem_ld_wait(o);
                 }
-                if (live) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t r[4];
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t r[4];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            r[x] = any ? pack16<BF16>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv) : 0u;
-                        *reinterpret_cast<uint4 *>(dst + 64 * i + 2 * e) = make_uint4(r[0], r[1], r[2], r[3]);
-                    }
+                    for (int x = 0; x < 4; ++x)
+                        r[x] = any ? pack16<BF16>(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv) : 0u;
+                    sts128(stage + lane * 256 + ((4 * i + e) ^ turn) * 16, r[0], r[1], r[2], r[3]);
                 }
+            }
+            const uint64_t dst = reinterpret_cast<uint64_t>(a.out) + 2 * ((a.cu_seqlens ? 0 : b) * a.ob + head * a.oh + (int64_t)(t0 + pos) * a.ot);
+            const uint64_t to = live ? dst : 0;
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < 32; i += 2) {
+                const int from = i + (lane >> 4);
+                uint4 *const row_to = reinterpret_cast<uint4 *>(__shfl_sync(0xffffffffu, to, from));
+                const uint4 v = lds128(stage + from * 256 + ((lane & 15) ^ (from & 15)) * 16);
+                if (row_to) row_to[lane & 15] = v;
             }
         }
     }

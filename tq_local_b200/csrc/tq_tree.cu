@@ -47,8 +47,10 @@ struct TreeArgs {
     const void *q;
     void *out;
     int64_t qb, qh, qt, ob, oh, ot;
-    uint16_t *qop;    // [batch][kv_heads][tiles][rows][128 or 256] fp16
-    float *part_ml, *part_o;  // [piece][rows][2], [piece][rows][128]
+    // Scratch, with a tile's rows innermost: lanes hold rows, and their 16 bytes lie side by side.
+    uint4 *qop;       // [tile][16 or 32][rows] fp16, eight coordinates each
+    float *part_ml;   // [piece][rows][2]
+    float4 *part_o;   // [piece][32][rows]
     int ctas;
     int *error_flag;
 };
@@ -232,9 +234,9 @@ template <typename T, bool QJL> __global__ void __launch_bounds__(kRowThreads, 1
     for (int e = 0; e < 16; ++e)
         o[e] = half2_bits(__uint_as_float(sketch ? y[e] : y[2 * e]) * f, __uint_as_float(sketch ? y[e + 16] : y[2 * e + 1]) * f);
     if (mine) {
-        uint4 *dst = reinterpret_cast<uint4 *>(a.qop + r * kWide + (sketch ? 128 : 0) + 32 * part);
+        const int64_t to = r / a.rows * (kWide / 8) + (sketch ? 16 : 0) + 4 * part;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dst[turned(part, e)] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        for (int e = 0; e < 4; ++e) a.qop[(to + turned(part, e)) * a.rows + r % a.rows] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
     }
     tile.finish(a.error_flag);
 }
@@ -538,11 +540,11 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             const uint64_t mask = live && a.mask ? a.mask[(int64_t)g.b * a.nodes + node] & (~0ull >> (64 - a.nodes)) : 0;
             const int chain_end = a.mask ? -1 : live ? node + 1 : 0;
             // ---- the queries (the products that read the ones before are done: their logits were here)
-            const uint4 *src = reinterpret_cast<const uint4 *>(a.qop + (g.tile * a.rows + row) * kWide) + kWide / 16 * half;
+            const uint4 *src = a.qop + (g.tile * (kWide / 8) + kWide / 16 * half) * a.rows + row;
             uint32_t q[kWide / 4];
 #pragma unroll
             for (int e = 0; e < kWide / 16; ++e) {
-                const uint4 x = row < a.rows ? src[e] : make_uint4(0, 0, 0, 0);
+                const uint4 x = row < a.rows ? src[e * a.rows] : make_uint4(0, 0, 0, 0);
                 q[4 * e] = x.x, q[4 * e + 1] = x.y, q[4 * e + 2] = x.z, q[4 * e + 3] = x.w;
             }
             __syncwarp();
@@ -647,7 +649,9 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                 tmem_ld_wait(o);
                 if (live)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(a.part_o + r * TQ_D + 64 * half + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 8; ++e)
+                        a.part_o[((g.tile + blockIdx.x) * 32 + 16 * half + 8 * i + e) * a.rows + row] =
+                            make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
             }
             umma_fence_before();
             pair_sync();  // (the sums have been read)
@@ -701,7 +705,7 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
         for (int b = 0; b < p.b; ++b) first += entry_length(a, cut, b);
         for (int x = 0; x < t; ++x) first += cut.length(tile_blocks(a, e, x));
         const int64_t c0 = first / cut.chunk;
-        piece0 = (p.tile + c0) * a.rows + p.in, n = (int)((first + nb - 1) / cut.chunk - c0) + 1;
+        piece0 = p.tile + c0, n = (int)((first + nb - 1) / cut.chunk - c0) + 1;
     }
     tq_grid_dependency_wait();
     float o[32] = {};
@@ -709,12 +713,11 @@ template <typename T> __global__ void __launch_bounds__(kRowThreads, 1) tq_tree_
     if (p.live) {
 #pragma unroll 2
         for (int c = group; c < n; c += groups) {
-            const int64_t piece = piece0 + (int64_t)c * a.rows;
-            const float2 x = reinterpret_cast<const float2 *>(a.part_ml)[piece];
-            const float4 *src = reinterpret_cast<const float4 *>(a.part_o + piece * TQ_D + 32 * part);
+            const float2 x = reinterpret_cast<const float2 *>(a.part_ml)[(piece0 + c) * a.rows + p.in];
+            const float4 *src = a.part_o + ((piece0 + c) * 32 + 8 * part) * a.rows + p.in;
             float4 v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = src[2 * turned(part, i >> 1) + (i & 1)];
+            for (int i = 0; i < 8; ++i) v[i] = src[(2 * turned(part, i >> 1) + (i & 1)) * a.rows];
             if (x.y == 0.f) continue;  // (a piece in which the row saw nothing)
             const float top = fmaxf(m, x.x), keep = exp2f(m - top), f = exp2f(x.x - top);
             m = top, l = l * keep + f * x.y;
@@ -894,8 +897,8 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v;
     a.q = q->data, a.qb = q->stride_b, a.qh = q->stride_h, a.qt = q->stride_t;
     a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
-    a.qop = reinterpret_cast<uint16_t *>(ws + p.qop);
-    a.part_ml = reinterpret_cast<float *>(ws + p.ml), a.part_o = reinterpret_cast<float *>(ws + p.o);
+    a.qop = reinterpret_cast<uint4 *>(ws + p.qop);
+    a.part_ml = reinterpret_cast<float *>(ws + p.ml), a.part_o = reinterpret_cast<float4 *>(ws + p.o);
     a.error_flag = ctx->error_flag;
     TQ_CUDA_CHECK(q->dtype == TQ_DTYPE_F16 ? launch<__half>(a, ctx, n_rows, (cudaStream_t)stream)
                                            : launch<__nv_bfloat16>(a, ctx, n_rows, (cudaStream_t)stream));
