@@ -14,8 +14,8 @@
 // are outside the sequence.  S = Q K^T with both operands in shared memory; the weights go back to TMEM over S as 16-bit pairs and are the A
 // operand of O += P V.  TMEM: S of the two tiles, O of the two tiles, 128 columns each.
 //
-// What bounds it: 32768 tokens, 32 / 8 heads, bf16, take 7.2 ms on a card at rest (1220 TFLOP/s) and 8.3 ms back to back, where the card's
-// power limit lowers its clock (1060; the library's matrix product falls from 1657 to 1376).  Between steps the tensor core waits for exponentials
+// What bounds it: 32768 tokens, 32 / 8 heads, bf16, take 7.3 ms on a card at rest (1200 TFLOP/s) and 8.4 ms back to back, where the card's
+// power limit lowers its clock (1050; the library's matrix product falls from 1657 to 1376).  Between steps the tensor core waits for exponentials
 // (16 a clock and SM against 8192 operations: as long as the products) and for the hand-over of logits and weights.
 #include <cuda.h>
 #include <math.h>
@@ -327,29 +327,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             umma_fence_after();
         }
-        const int head = h * a.group + row % a.group;
+        const int head = h * a.group + row % a.group, lane = tid & 31;
+        // Rows leave through the tile's query image, which nobody reads any more, sixteen lanes to a row: a warp's 32 rows of 256 bytes, 16-byte
+        // pieces turned by the row.
+        const uint32_t stage = base + w * kSlotBytes + (warp & 3) * 32 * 256, turn = lane & 15;
+        auto copy_rows = [&](uint64_t to) {  // this lane's row goes to `to` (0: nowhere)
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < 32; i += 2) {
+                const int from = i + (lane >> 4);
+                const uint64_t row_to = __shfl_sync(0xffffffffu, to, from);
+                const uint4 v = lds128(stage + from * 256 + ((lane & 15) ^ (from & 15)) * 16);
+                if (row_to) reinterpret_cast<uint4 *>(row_to)[lane & 15] = v;
+            }
+            __syncwarp();
+        };
         if (a.splits > 1) {
             const int64_t r = (((int64_t)b * a.n_q + pos) * (a.kv_heads * a.group) + head) * a.splits + blockIdx.y;
             if (live) a.part_ml[2 * r] = m_ref * c, a.part_ml[2 * r + 1] = l;
-            if (mine) {
+            if (mine) {  // (half of the coordinates at a time, the way the finished rows go, see below)
+                const uint64_t to = live ? reinterpret_cast<uint64_t>(a.part_o + r * TQ_D) : 0;
 #pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t o[32];
-                    __syncwarp();
-                    tmem_ld32(t_o + 32 * i, o);
-                    tmem_ld_wait(o);
-                    if (live)
+                for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(a.part_o + r * TQ_D + 32 * i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t o[32];
+                        __syncwarp();
+                        tmem_ld32(t_o + 64 * i + 32 * x, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sts128(stage + lane * 256 + ((8 * x + e) ^ turn) * 16, o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                    copy_rows(to ? to + 256 * i : 0);
                 }
             }
         } else {
-            // Rows leave through the tile's query image, which nobody reads any more, sixteen lanes to a row: a warp's 32 rows of 256 bytes, 16-byte
-            // pieces turned by the row.
             const bool any = l > 0.f || l != l;
             const float inv = any ? 1.f / l : 0.f;
-            const int lane = tid & 31;
-            const uint32_t stage = base + w * kSlotBytes + (warp & 3) * 32 * 256, turn = lane & 15;
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 uint32_t o[32] = {};
@@ -368,15 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const uint64_t dst = reinterpret_cast<uint64_t>(a.out) + 2 * ((a.cu_seqlens ? 0 : b) * a.ob + head * a.oh + (int64_t)(t0 + pos) * a.ot);
-            const uint64_t to = live ? dst : 0;
-            __syncwarp();
-#pragma unroll 4
-            for (int i = 0; i < 32; i += 2) {
-                const int from = i + (lane >> 4);
-                uint4 *const row_to = reinterpret_cast<uint4 *>(__shfl_sync(0xffffffffu, to, from));
-                const uint4 v = lds128(stage + from * 256 + ((lane & 15) ^ (from & 15)) * 16);
-                if (row_to) row_to[lane & 15] = v;
-            }
+            copy_rows(live ? dst : 0);
         }
     }
     if (lost) atomicExch(&g_prompt_status, 1);
@@ -431,22 +437,28 @@ int sm_count() {
     return n;
 }
 
-// Two tiles a CTA as soon as one each would not fit the SMs at a time.  Where even those leave SMs idle, the keys are cut: a block of keys
-// takes a CTA about a microsecond and joining the pieces a launch, so a piece has at least four blocks.
+// One tile a CTA or two, and into how many pieces its keys are cut: what takes the least time by three figures.  A block of keys takes a CTA 1.5 us
+// with one tile and 2.3 with two (whose products and exponentials go on beside each other), starting and ending one 4, joining pieces 6 (512 queries
+// behind 16384 keys, 32 / 8 heads: 197 us with one tile and one piece, 141 as chosen here: two tiles, two pieces).  Under a causal mask a tile sees the keys before
+// the queries and half of theirs on average.
 struct Plan {
     int positions, tiles_per_cta, n_items, splits;
 };
 Plan plan(int64_t batch, int q_heads, int kv_heads, int n_q, int n_kv) {
-    Plan p;
-    p.positions = kUmmaRows / (q_heads / kv_heads);
-    const int sms = sm_count(), tiles = (n_q + p.positions - 1) / p.positions;
-    p.tiles_per_cta = batch * kv_heads * tiles > sms ? 2 : 1;
-    p.n_items = (tiles + p.tiles_per_cta - 1) / p.tiles_per_cta;
-    const int64_t ctas = batch * kv_heads * p.n_items;
-    const int blocks = (n_kv + kBlock - 1) / kBlock;
-    p.splits = ctas && ctas <= sms / 2 ? (int)(sms / ctas < blocks / 4 ? sms / ctas : blocks / 4) : 1;
-    if (p.splits < 1) p.splits = 1;
-    return p;
+    Plan best = {};
+    const int positions = kUmmaRows / (q_heads / kv_heads), sms = sm_count(), tiles = (n_q + positions - 1) / positions;
+    const int blocks = n_kv >= n_q ? (n_kv - n_q / 2 + kBlock - 1) / kBlock : (n_kv + kBlock - 1) / kBlock;
+    double least = 0;
+    for (int two = 1; two <= 2; ++two) {
+        const int items = (tiles + two - 1) / two;
+        const int64_t ctas = batch * kv_heads * items;
+        for (int splits = 1; splits <= 32 && (splits == 1 || (ctas * splits <= sms && splits <= blocks / 2)); ++splits) {
+            const int64_t rounds = (ctas * splits + sms - 1) / sms;
+            const double time = rounds * ((blocks + splits - 1) / splits * (two == 2 ? 2.3 : 1.5) + 4.0) + (splits > 1 ? 6.0 : 0.0);
+            if (!best.positions || time < least) best = {positions, two, items, splits}, least = time;
+        }
+    }
+    return best;
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
