@@ -22,6 +22,29 @@ def desc(data=4096, dtype=1, b=8 * 128, h=128, t=128):
     return C.byref(DenseDesc(data, dtype, b, h, t))
 
 
+def test_prompt_kernels_replace_sdpa_alone():
+    """Another implementation may add terms that neither the kernels nor their fall-back compute."""
+    from types import SimpleNamespace
+
+    from tq_local_b200.runtime.generation import _prompt_kernels
+
+    ids = torch.zeros(2, 4, dtype=torch.long)
+    inside = lambda mask=None, enabled=True, **config: _inside(_prompt_kernels, SimpleNamespace(config=SimpleNamespace(**config)),
+                                                                {"input_ids": ids, "attention_mask": mask}, enabled)
+    assert inside(_attn_implementation="sdpa") == ("turboquant_prompt", "sdpa")
+    assert inside(_attn_implementation="sdpa", enabled=False) == ("sdpa", "sdpa")
+    assert inside(_attn_implementation="eager") == ("eager", "eager")
+    assert inside(_attn_implementation="sdpa", attention_chunk_size=8192) == ("sdpa", "sdpa")
+    assert inside(torch.tensor([[0, 0, 1, 1], [1, 1, 1, 1]]), _attn_implementation="sdpa") == ("turboquant_prompt", "sdpa")
+    assert inside(torch.tensor([[1, 0, 1, 1], [1, 1, 1, 1]]), _attn_implementation="sdpa") == ("sdpa", "sdpa")
+
+
+def _inside(manager, model, inputs, enabled):
+    with manager(model, inputs, enabled):
+        seen = model.config._attn_implementation
+    return seen, model.config._attn_implementation
+
+
 def test_prompt_refuses_bad_arguments():
     d = desc()
     call = lambda q=d, k=d, v=d, b=1, hq=4, hkv=2, n=8, m=8, start=None, out=d, ws=None, size=0, causal=1: lib().tq_prompt_attn(

@@ -102,17 +102,19 @@ def _prefill(model, inputs, cache=None):
 @contextmanager
 def _prompt_kernels(model, inputs, enabled: bool):
     """The prompt pass inside runs on this library's prompt attention where it computes what the model asks for (see
-    ``prompt_attention.turboquant_prompt_forward``).  Only causal, at most left-padded batches qualify."""
+    ``prompt_attention.turboquant_prompt_forward``).  Only causal, at most left-padded batches of models that run ``sdpa`` qualify: what
+    the kernels do not compute goes there, and another implementation may add terms (soft-capped logits, sinks) that it does not."""
     from tq_local_b200.runtime.packed_qmse_cache import is_left_padding_mask
 
     config, mask = getattr(model, "config", None), inputs.get("attention_mask")
-    if not enabled or config is None or (mask is not None and not is_left_padding_mask(mask)):
+    previous = getattr(config, "_attn_implementation", None)
+    if (not enabled or config is None or previous not in (None, "sdpa") or getattr(config, "attention_chunk_size", None)
+            or (mask is not None and not is_left_padding_mask(mask))):
         yield
         return
     from tq_local_b200.runtime.prompt_attention import raise_on_status, register_prompt_backend
 
     register_prompt_backend()
-    previous = getattr(config, "_attn_implementation", None)
     config._attn_implementation = "turboquant_prompt"
     try:
         yield
