@@ -541,3 +541,38 @@ def test_hooks_of_layers_with_a_dense_tail_and_of_dense_layers():
         assert layer.get_seq_length() == 10 and layer._dense_k.length == (10 if dense_layer else 0)
         layer.batch_repeat_interleave(2)
         assert (layer._dense_k.buf if dense_layer else layer.store.k_codes).shape[0] == 4
+
+
+def test_rows_of_a_padded_cache_are_not_recorded():
+    """The row offsets go to a tensor of their own, which a replay would fill from the old ones again; without offsets a replay moves rows again."""
+    from tq_local_b200.runtime import ffi
+
+    store = make_store(4, True, 3, 2, 24)
+    index = torch.tensor([1, 2, 0], device="cuda")
+    store.select_rows(index)  # (loads the kernel)
+    before = store.k_codes.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        store.select_rows(index)
+    graph.replay(), graph.replay()
+    assert torch.equal(store.k_codes, before[index][index])
+    starts = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda")
+    store.set_seq_start(starts)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ffi.TQError):
+            store.select_rows(index)
+    store.select_rows(index)
+    assert store._seq_start.tolist() == [3, 5, 0] and starts.tolist() == [0, 3, 5]
+
+
+def test_more_rows_in_place_than_fit_are_refused():
+    import ctypes as C
+
+    from tq_local_b200.runtime import ffi
+
+    store = make_store(4, True, 2, 2, 24)
+    for rows in (449, 4_194_304, 8_388_608):  # refused on the host, before anything is read
+        d = ffi.CacheDesc.from_buffer_copy(store._desc_ref._obj)
+        d.batch = rows
+        assert ffi.lib().tq_cache_select_rows(store.codec.handle, C.byref(d), C.byref(d), store.k_codes.data_ptr(), 0, 24, None, None) == -2

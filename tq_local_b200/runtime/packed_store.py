@@ -459,7 +459,7 @@ class PackedStore:
         """Move the accepted drafted tokens behind their histories: token ``tree_start + path[b, i]`` of row ``b`` goes to token
         ``lengths[b] + i`` for ``i < counts[b]`` (``path`` int32 [B, P], ascending in every row; ``counts``, ``lengths`` int32
         [B]).  Returns the new lengths, int32 [B]; ``length`` is the host's to set (``truncate``) once it knows the longest.
-        A row whose path or length is out of range stays as it is and is reported (device status 7)."""
+        A row whose path leaves the cache's capacity, or whose count or length is out of range, stays as it is and is reported (device status 7)."""
         b = self.batch
         if path.dim() != 2:
             raise ValueError(f"path must be an int32 tensor [{b}, P]")
@@ -495,6 +495,8 @@ class PackedStore:
         hi = self.length if hi is None else int(hi)
         if index.numel() != self.batch or not 0 <= int(lo) <= hi <= self.length:
             raise ValueError(f"select_rows takes {self.batch} rows and tokens within [0, {self.length}), got {index.numel()} and [{lo}, {hi})")
+        if self._seq_start is not None and torch.cuda.is_current_stream_capturing():
+            raise ffi.TQError("select_rows gives a left-padded cache new offsets: a replayed graph would start from the old ones")
         starts = None if self._seq_start is None else torch.empty_like(self._seq_start)
         ffi.launch("tq_cache_select_rows", self.codec.device, (
             self.codec.handle, self._desc_ref, self._desc_ref, index.data_ptr(), int(lo), hi, None if starts is None else starts.data_ptr()))
