@@ -97,6 +97,19 @@ def test_rows_that_kernels_cannot_address_are_copied():
     assert (d.stride_b, d.stride_h, d.stride_t) == (0, 0, 0)
 
 
+def test_operands_are_aligned_views_with_their_strides():
+    from tq_local_b200.runtime.codec import aligned_view, operand, strided_desc
+
+    x = torch.zeros(2, 3, 4, 256, dtype=torch.bfloat16)
+    for t in (x[..., :128], x[..., ::2], x[..., 1:129], x[:, :1, :, :128].expand(2, 3, 4, 128), x[:1, :, :1, :128], x[..., :128].transpose(1, 2),
+              torch.zeros(2, 3, 4, 129, dtype=torch.float16)[..., :128], torch.zeros(5, 129, dtype=torch.float16)[:1, :128].view(1, 1, 1, 128)):
+        view, d = operand(t)
+        same = aligned_view(t)
+        assert (view is t) == (same is t) and view.stride() == same.stride()
+        want = strided_desc(view)
+        assert [getattr(d, name) for name, _ in d._fields_] == [getattr(want, name) for name, _ in d._fields_]
+
+
 def test_dense_rows_follow_an_index():
     from tq_local_b200.runtime.packed_qmse_cache import _GrowingDense
 

@@ -66,6 +66,16 @@ def strided_desc(t: torch.Tensor) -> ffi.DenseDesc:
     return ffi.DenseDesc(t.data_ptr(), _TORCH_TO_TQ[t.dtype], sb if b > 1 else 0, sh if h > 1 else 0, st if n > 1 else 0)
 
 
+def operand(t: torch.Tensor) -> tuple[torch.Tensor, ffi.DenseDesc]:
+    """``aligned_view`` of a 16-bit [B, H, T, 128] that is not empty and its ``strided_desc``, in one look at the strides (small calls are bound by their
+    host work)."""
+    (b, h, n, _), (sb, sh, st, last), data = t.shape, t.stride(), t.data_ptr()
+    sb, sh, st = (sb or 1) if b > 1 else 0, (sh or 1) if h > 1 else 0, (st or 1) if n > 1 else 0  # (an axis repeated by 0 is copied: 1 is no multiple of 8)
+    if last != 1 or data & 15 or (sb | sh | st) & 7:
+        return operand(t.clone(memory_format=torch.contiguous_format))
+    return t, ffi.DenseDesc(data, _TORCH_TO_TQ[t.dtype], sb, sh, st)
+
+
 def refuse_grad(what: str, *tensors: torch.Tensor) -> None:
     if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
         raise ffi.TQError(f"{what} has no backward pass: call it under torch.no_grad() or on detached tensors")

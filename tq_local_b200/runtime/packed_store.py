@@ -23,7 +23,7 @@ import ctypes as C
 import torch
 
 from tq_local_b200.runtime import ffi
-from tq_local_b200.runtime.codec import Codec, aligned_view, dense_desc, refuse_grad, strided_desc, tq_dtype
+from tq_local_b200.runtime.codec import Codec, aligned_view, dense_desc, operand, refuse_grad, strided_desc, tq_dtype
 
 
 def _round_up(n: int, m: int) -> int:
@@ -441,15 +441,14 @@ class PackedStore:
                 raise ValueError(f"tree_mask must be an int64 tensor [{b}, {t}] or [{t}] on {self.codec.device}")
             tree_mask = (tree_mask if tree_mask.dim() == 2 else tree_mask.expand(b, t)).contiguous()
         if out is None:
-            out = torch.empty(b, t, hq, 128, dtype=q.dtype, device=q.device).transpose(1, 2)
+            out = torch.empty_strided((b, hq, t, 128), (t * hq * 128, 128, hq * 128, 1), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or aligned_view(out) is not out:
             raise ValueError("out must have the queries' shape, dtype and device, with rows on 16-byte boundaries")
         if t == 0:
             return out
-        q = aligned_view(q)
         need = int(ffi.lib().tq_tree_workspace_bytes(self.codec.handle, b, hq, self.kv_heads, t, start))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # (the call's own: calls may overlap or be recorded)
-        qd, od = strided_desc(q), strided_desc(out)
+        (q, qd), od = operand(q), strided_desc(out)
         ffi.launch("tq_tree_attn", self.codec.device, (
             self.codec.handle, C.byref(qd), hq, t, self._desc_ref, start, None if lengths is None else lengths.data_ptr(),
             None if tree_mask is None else tree_mask.data_ptr(), ws.data_ptr(), need, C.byref(od)))

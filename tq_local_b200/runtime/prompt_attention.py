@@ -12,7 +12,7 @@ import ctypes as C
 import torch
 
 from tq_local_b200.runtime import ffi
-from tq_local_b200.runtime.codec import aligned_view, refuse_grad, strided_desc
+from tq_local_b200.runtime.codec import aligned_view, operand, refuse_grad, strided_desc
 
 
 _SCALE = 128 ** -0.5
@@ -68,13 +68,13 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         raise ValueError(f"keys {tuple(key.shape)} do not go with queries {tuple(query.shape)}" + (" under a causal mask" if causal else ""))
     if seq_start is not None:
         seq_start = _int32(seq_start, (b,), query.device, "seq_start")
-    out = _output(out, query, lambda: torch.empty(b, n_q, hq, 128, dtype=query.dtype, device=query.device).transpose(1, 2))
+    out = _output(out, query, lambda: torch.empty_strided((b, hq, n_q, 128), (n_q * hq * 128, 128, hq * 128, 1), dtype=query.dtype,
+                                                          device=query.device))
     if out.numel() == 0:
         return out
     if n_kv == 0:
         return out.zero_()
-    q, k, v = aligned_view(query), aligned_view(key), aligned_view(value)
-    qd, kd, vd, od = strided_desc(q), strided_desc(k), strided_desc(v), strided_desc(out)
+    (q, qd), (k, kd), (v, vd), od = operand(query), operand(key), operand(value), strided_desc(out)
     ws, need = _workspace(query.device, b, hq, hkv, n_q, n_kv)
     ffi.launch("tq_prompt_attn", query.device, (
         C.byref(qd), C.byref(kd), C.byref(vd), b, hq, hkv, n_q, n_kv, None if seq_start is None else seq_start.data_ptr(),
@@ -97,8 +97,8 @@ def prompt_attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch
     out = _output(out, query, lambda: torch.empty(total, hq, 128, dtype=query.dtype, device=query.device))
     if n == 0 or max_seqlen == 0:
         return out
-    q, k, v = aligned_view(query), aligned_view(key), aligned_view(value)
-    qd, kd, vd, od = (strided_desc(t.transpose(0, 1).unsqueeze(0)) for t in (q, k, v, out))
+    (q, qd), (k, kd), (v, vd) = (operand(t.transpose(0, 1).unsqueeze(0)) for t in (query, key, value))
+    od = strided_desc(out.transpose(0, 1).unsqueeze(0))
     ws, need = _workspace(query.device, n, hq, hkv, int(max_seqlen), int(max_seqlen))
     ffi.launch("tq_prompt_attn_packed", query.device, (
         C.byref(qd), C.byref(kd), C.byref(vd), n, total, hq, hkv, cu_seqlens.data_ptr(), int(max_seqlen),
