@@ -576,3 +576,12 @@ def test_more_rows_in_place_than_fit_are_refused():
         d = ffi.CacheDesc.from_buffer_copy(store._desc_ref._obj)
         d.batch = rows
         assert ffi.lib().tq_cache_select_rows(store.codec.handle, C.byref(d), C.byref(d), store.k_codes.data_ptr(), 0, 24, None, None) == -2
+
+
+@pytest.mark.parametrize("name", ["k_norms", "k_rnorms", "v_norms"])
+def test_nan_norms_reach_the_head_that_holds_them_alone(name):
+    store = make_store(4, True, 2, 2, 700)
+    q = queries(2, 8, 5, F16)
+    getattr(store, name)[1, 0, 130] = math.nan
+    out = store.tree_attn(q)
+    assert out[1, :4].isnan().all() and out[0].isfinite().all() and out[1, 4:].isfinite().all()

@@ -334,3 +334,19 @@ def test_refusals():
     assert (prompt_attention(q, k[:, :, :0], v[:, :, :0], causal=False) == 0).all()
     assert prompt_attention(q[:0], k[:0], v[:0]).shape == (0, 4, 8, 128)
     assert prompt_attention_packed(*p, cu[:1], 0).shape == p[0].shape
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_nan_keys_reach_the_queries_that_see_them_and_no_others(dtype):
+    """One NaN key at each place of a block, a batch entry each: what sees it is NaN, what comes before it is not."""
+    from tq_local_b200.runtime.prompt_attention import prompt_attention
+
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(128, 1, 300, 128, device="cuda", generator=gen).to(dtype) for _ in range(3))
+    at = torch.arange(128, device="cuda")
+    k[at, 0, at, 7] = math.nan
+    out = prompt_attention(q, k, v)
+    sees = torch.arange(300, device="cuda")[None, :] >= at[:, None]
+    assert out[:, 0].isnan().all(-1).equal(sees) and out[:, 0].isfinite().all(-1).equal(~sees)
+    few = prompt_attention(q[:2, :, -3:], k[:2], v[:2])  # pieces of the keys, joined
+    assert few.isnan().all()

@@ -119,9 +119,10 @@ __device__ __forceinline__ void exp2_poly(uint64_t x2, float &p, float &q) {
     uint64_t y = f32x2_fma(f32x2(0.0551716685f, 0.0551716685f), f, f32x2(0.242611125f, 0.242611125f));
     y = f32x2_fma(y, f, f32x2(0.693260968f, 0.693260968f));
     y = f32x2_fma(y, f, f32x2(0.999928057f, 0.999928057f));
-    float na, nb, ya, yb;
-    f32x2_split(n, na, nb), f32x2_split(y, ya, yb);
-    p = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(na) << 23)), q = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(nb) << 23));
+    float na, nb;
+    f32x2_split(n, na, nb);
+    const float pa = __uint_as_float((__float_as_uint(na) << 23) + 0x3f800000u), pb = __uint_as_float((__float_as_uint(nb) << 23) + 0x3f800000u);
+    f32x2_split(f32x2_mul(y, f32x2(pa, pb)), p, q);  // (a product: NaN stays NaN, which adding to its exponent field would not leave)
 }
 // The running maximum that a row's weights are relative to may lag behind the true one by up to 2^kLag: fp16 weights stay below
 // 2^9 and the sums far from overflow, and the accumulator is rescaled a few times a row instead of at every block.
