@@ -116,14 +116,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     }
-    if (tid == 0) {
+    // copies: Q0, K0, Q1, V0, K1, V1, ...; the first ones, which wait for no free slot, leave before the CTA has set up the rest
+    auto load_q = [&](int w) {
+        mbar_expect_tx(bar_q + 8 * w, 256 * a.positions * a.group);
+        for (int x = 0; x < 2; ++x)
+            load_map(base + w * kSlotBytes + x * kUmmaSlabBytes, &map_q, bar_q + 8 * w, 64 * x, 0, t0 + first_pos + w * a.positions, h, a.cu_seqlens ? 0 : b);
+    };
+    auto load_slot = [&](int i) {  // keys of block i / 2, or its values
+        const int slot = i % kSlots;
+        const uint32_t bar = bar_full + 8 * slot;
+        mbar_expect_tx(bar, kSlotBytes);
+        for (int x = 0; x < 2; ++x)
+            load_map(ring + slot * kSlotBytes + x * kUmmaSlabBytes, i & 1 ? &map_v : &map_k, bar, 64 * x, t0 + (first_block + i / 2) * kBlock, h, a.cu_seqlens ? 0 : b);
+    };
+    if (warp == kSoftmax / 32 && elect_one()) {
         mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1), mbar_init(bar_ask, 1), mbar_init(bar_clean, 1), mbar_init(bar_clean + 8, 1);
         for (int i = 0; i < 4; ++i) mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 4);
         for (int w = 0; w < 2; ++w) mbar_init(bar_o + 8 * w, 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        if (nu0) load_q(0);
+        for (int i = 0; i < min(2 * nb, kSlots); ++i) {
+            load_slot(i);
+            if (i == 0 && nu1) load_q(1);
+        }
     }
+    __syncwarp();
     umma_fence_before();
     __syncthreads();
     umma_fence_after();
@@ -138,23 +157,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp >= kSoftmax / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
         if (warp == kSoftmax / 32) {
-            // ---------------- copies: Q0, K0, Q1, V0, K1, V1, ...
+            // ---------------- copies
             if (elect_one()) {
-                const int bb = a.cu_seqlens ? 0 : b;
-                auto load_q = [&](int w) {
-                    mbar_expect_tx(bar_q + 8 * w, 256 * a.positions * a.group);
-                    for (int x = 0; x < 2; ++x)
-                        load_map(base + w * kSlotBytes + x * kUmmaSlabBytes, &map_q, bar_q + 8 * w, 64 * x, 0, t0 + first_pos + w * a.positions, h, bb);
-                };
-                if (nu0) load_q(0);
-                for (int i = 0; i < 2 * nb; ++i) {
-                    const int slot = i % kSlots;
-                    wait(bar_empty + 8 * slot, (i / kSlots & 1) ^ 1);
-                    const uint32_t bar = bar_full + 8 * slot;
-                    mbar_expect_tx(bar, kSlotBytes);
-                    for (int x = 0; x < 2; ++x)
-                        load_map(ring + slot * kSlotBytes + x * kUmmaSlabBytes, i & 1 ? &map_v : &map_k, bar, 64 * x, t0 + (first_block + i / 2) * kBlock, h, bb);
-                    if (i == 0 && nu1) load_q(1);
+                for (int i = kSlots; i < 2 * nb; ++i) {
+                    wait(bar_empty + 8 * (i % kSlots), (i / kSlots & 1) ^ 1);
+                    load_slot(i);
                 }
             }
         } else if (warp < kSoftmax / 32 + 3) {
