@@ -14,6 +14,10 @@
 // half the odd ones.  Warp 24 issues the products, S = [Rq | Sq] [K | signs]^T with the queries in TMEM and O += P V.  Warp 25 requests the packed
 // blocks (bulk copies, a ring of three).  TMEM: S of two blocks, O, the queries, 128 columns each.
 //
+// Roundings to fp16: the rotated queries, a centre, a centre times its norm, a weight; everything else is fp32.  With fp16 outputs the error is
+// 8e-4 relative to 64 bits (the output's own rounding 2e-4), with bf16 outputs 1.8e-3 (1.7e-3).  The largest share is that of the key operands: with the
+// norms multiplied onto fp32 logits instead it is 5.5e-4, and 16 nodes over 8 x 32768 tokens take 221 us instead of 192.
+//
 // What bounds it: a block of 128 tokens takes a CTA 1.6 to 1.7 us whatever the bits, the sketch and the number of rows.  Of 195 us for 16 nodes over
 // 8 x 32768 tokens (32 / 8 heads, 4 bits, sketch) leaving out the operands' stores gives back 48, the products 28, the look-ups 25, the exponentials 5; with
 // all four left out 109 remain, which is the hand-over from role to role.  Shared memory is three quarters busy (operands written once and read once by the
@@ -531,16 +535,8 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         constexpr int kWide = QJL ? 256 : 128;
         // the two warps that share 32 rows
         auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + (warp & 3)) : "memory"); };
-        uint32_t n = 0;
-        tq_grid_dependency_wait();  // (the queries)
-        if ((warp & 3) < row_warps) while (flat < flat_end) {
-            const Segment g = next_segment();
-            const int node = g.t * a.positions + row / a.group;
-            const bool live = row < a.rows && node < a.nodes;
-            const uint64_t mask = live && a.mask ? a.mask[(int64_t)g.b * a.nodes + node] & (~0ull >> (64 - a.nodes)) : 0;
-            const int chain_end = a.mask ? -1 : live ? node + 1 : 0;
-            // ---- the queries (the products that read the ones before are done: their logits were here)
-            const uint4 *src = a.qop + (g.tile * (kWide / 8) + kWide / 16 * half) * a.rows + row;
+        auto load_queries = [&](int64_t t) {  // of tile t
+            const uint4 *src = a.qop + (t * (kWide / 8) + kWide / 16 * half) * a.rows + row;
             uint32_t q[kWide / 4];
 #pragma unroll
             for (int e = 0; e < kWide / 16; ++e) {
@@ -553,6 +549,18 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             tmem_st_wait();
             umma_fence_before();
             mbar_arrive_warp(bar_q);
+        };
+        uint32_t n = 0;
+        tq_grid_dependency_wait();  // (the queries)
+        const bool any = (warp & 3) < row_warps && flat < flat_end;
+        Segment next = {};
+        if (any) next = next_segment(), load_queries(next.tile);
+        if (any) for (bool more = true; more;) {
+            const Segment g = next;
+            const int node = g.t * a.positions + row / a.group;
+            const bool live = row < a.rows && node < a.nodes;
+            const uint64_t mask = live && a.mask ? a.mask[(int64_t)g.b * a.nodes + node] & (~0ull >> (64 - a.nodes)) : 0;
+            const int chain_end = a.mask ? -1 : live ? node + 1 : 0;
             float m_ref = -INFINITY;
             uint64_t sum[2] = {0, 0};
             for (int k = g.k; k < g.k_end; ++k, ++n) {
@@ -629,6 +637,9 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                 if (k > g.k && k + 1 == g.k_end) wait(bar_o, (n - 1) & 1);
                 mbar_arrive_warp(bar_p + 8 * (n & 1));
             }
+            // ---- the next queries, so that their first products run beside what follows (those that read the ones before are done: their logits were here)
+            more = flat < flat_end;
+            if (more) next = next_segment(), load_queries(next.tile);
             // ---- this piece of the tile's rows
             float l0, l1;
             f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
