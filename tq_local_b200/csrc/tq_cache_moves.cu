@@ -2,7 +2,7 @@
 // fork, requests that enter or leave a batch) and accepted drafted tokens that move behind their history.
 //
 // Both only carry bytes: six streams, in 16-byte units.  What bounds them is HBM for rows (16 rows of 8 heads x 32768 tokens, some of them copies of others,
-// 457 MB read and written in place: 86 us, 5.3 TB/s or 0.81 of a plain copy's rate) and the launch for few of either (100 tokens of four rows 2.9 us,
+// 457 MB read and written in place: 85 us, 5.4 TB/s or 0.82 of a plain copy's rate) and the launch for few of either (100 tokens of four rows 2.9 us,
 // 12 accepted tokens 4.8, 64 of 64 sequences 5.8, each in a recorded graph).
 #include "tq_common.cuh"
 
@@ -55,7 +55,8 @@ struct RowArgs {
     int *error_flag;
 };
 
-template <bool STAGED> __global__ void __launch_bounds__(128) tq_select_rows_kernel(const __grid_constant__ RowArgs a) {
+// (Five blocks an SM: the registers that this leaves a thread keep more of its loads in flight; the case above 89.5 us without, 87.5 with, as single calls.)
+template <bool STAGED> __global__ void __launch_bounds__(128, 5) tq_select_rows_kernel(const __grid_constant__ RowArgs a) {
     extern __shared__ uint4 stage[];  // [row][thread]
     const int h = blockIdx.y;
     int s = 0;
