@@ -288,7 +288,9 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 1 + 1 + 1 + 2 + 2 * kRingSlots];
     __shared__ uint32_t s_tmem;
-    __shared__ float s_half[2][kUmmaRows];
+    // What two warps that share rows tell each other, [block parity][half][row].  Two copies: one warp may be at the next block's logits while the other has
+    // not yet read the maximum of this one (the products for them do not wait for this block's weights), but no further ahead than that.
+    __shared__ float s_half[2][2][kUmmaRows];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = smem_u32(s_bars);
     // kfull, vfull: operands are there; kfree, vfree: the products that read keys and signs, or values, are done; s: logits are there; p: weights are there; o: O += P V is
@@ -589,11 +591,11 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                     for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
                 const float last = max3(__uint_as_float(s[60]), __uint_as_float(s[61]), fmaxf(__uint_as_float(s[62]), __uint_as_float(s[63])));
                 float peak = max3(max3(top[0], top[1], top[2]), top[3], last);
-                s_half[half][row] = peak;
+                s_half[n & 1][half][row] = peak;
                 umma_fence_before();
                 pair_sync();  // (both have read their logits as well: the weights go over them)
                 umma_fence_after();
-                peak = fmaxf(peak, s_half[half ^ 1][row]);
+                peak = fmaxf(peak, s_half[n & 1][half ^ 1][row]);
                 if (k == g.k) {
                     m_ref = peak;
                 } else {
@@ -644,9 +646,9 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             float l0, l1;
             f32x2_split(f32x2_add(sum[0], sum[1]), l0, l1);
             pair_sync();  // (the last peak has been read)
-            s_half[half][row] = l0 + l1;
+            s_half[0][half][row] = l0 + l1;
             pair_sync();
-            const float l = s_half[0][row] + s_half[1][row];
+            const float l = s_half[0][0][row] + s_half[0][1][row];
             wait(bar_o, (n - 1) & 1);
             __syncwarp();
             umma_fence_after();
