@@ -54,3 +54,15 @@ def test_halves_of_a_row_tell_each_other_the_maximum_of_the_same_block():
     assert len(uses) == 2
     copies = 2 if sizes == "[2][2][kUmmaRows]" and all(u.startswith("[n & 1]") for u in uses) else 1
     assert not exchange_goes_wrong(copies)
+
+
+def test_waits_for_tensor_memory_name_the_registers_that_arrive():
+    """A load from tensor memory is asynchronous: what does arithmetic on its registers must depend on the statement that waits, or the compiler may
+    move it ahead of that."""
+    found = 0
+    for name in sorted(os.listdir(CSRC)):
+        for statement in re.findall(r"asm volatile\(((?:[^;\"]|\"(?:[^\"\\]|\\.)*\")*)\);", source(name)):
+            if "tcgen05.wait::ld" in statement:
+                found += 1
+                assert "tcgen05.ld." in statement or '"+r"' in statement, (name, statement)
+    assert found == 2
