@@ -137,3 +137,24 @@ def test_maxima_that_move_from_block_to_block(bits, qjl, order, b, hkv, t):
     for _ in range(20):
         assert torch.equal(store.tree_attn(q), first)
     assert store.codec.device_status() == 0
+
+
+@pytest.mark.parametrize("bits,qjl", [(4, True), (3, False), (2, False)])
+@pytest.mark.parametrize("power", [-10, -12, -14, -16])
+@pytest.mark.parametrize("t", [1, 12])
+def test_small_values(bits, qjl, power, t):
+    """A cache whose values all have norms around 2^power: centres times norm would be among fp16's smallest numbers but for the factor 2^e."""
+    k, v = normal(2, 2, 300 + t, seed=3), normal(2, 2, 300 + t, seed=4) * (2.0 ** power / math.sqrt(128))
+    store = store_of(bits, qjl, k, v)
+    q = queries(2, 8, t, BF16)
+    check(store.tree_attn(q), *expected(store, q, 300))
+
+
+@pytest.mark.parametrize("bits,qjl", [(4, True), (3, False), (2, False)])
+def test_the_largest_values(bits, qjl):
+    """Norms up to fp16's largest number."""
+    k, v = normal(1, 2, 200, seed=3), normal(1, 2, 200, seed=4)
+    store = store_of(bits, qjl, k, v)
+    store.v_norms[:, :, ::3] = 65504.0
+    q = queries(1, 8, 5, BF16)
+    check(store.tree_attn(q), *expected(store, q, 195))

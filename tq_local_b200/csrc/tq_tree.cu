@@ -14,7 +14,9 @@
 // half the odd ones.  Warp 24 issues the products, S = [Rq | Sq] [K | signs]^T with the queries in TMEM and O += P V.  Warp 25 requests the packed
 // blocks (bulk copies, a ring of three).  TMEM: S of two blocks, O, the queries, 128 columns each.
 //
-// Roundings to fp16: the rotated queries, a centre, a centre times its norm, a weight; everything else is fp32.  With fp16 outputs the error is
+// Roundings to fp16: the rotated queries, a centre, a centre times its norm, a weight; everything else is fp32.  Value centres are taken times the power of two
+// that brings the largest to [1/2, 1): with the largest norm of fp16 they still fit, and norms down to 10^-4 stay clear of fp16's smallest numbers (a key
+// operand's lost bits are lost to a logit in absolute terms, where they are nothing).  With fp16 outputs the error is
 // 8e-4 relative to 64 bits (the output's own rounding 2e-4), with bf16 outputs 1.8e-3 (1.7e-3).  The largest share is that of the key operands: with the
 // norms multiplied onto fp32 logits instead it is 5.5e-4, and 16 nodes over 8 x 32768 tokens take 221 us instead of 192.
 //
@@ -48,6 +50,7 @@ struct TreeArgs {
     const uint16_t *image_k, *image_s, *image_v;  // R_k, S, R_v
     float unscale_k, unscale_s, unscale_v;
     const float *centers_k, *centers_v;
+    float cen_v_scale;  // power of two that brings the largest value centre to [1/2, 1), see the value operand
     const void *q;
     void *out;
     int64_t qb, qh, qt, ob, oh, ot;
@@ -314,7 +317,7 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     {
-        const float ck = a.centers_k[lane & 15], cv = a.centers_v[lane & 15];
+        const float ck = a.centers_k[lane & 15], cv = a.centers_v[lane & 15] * a.cen_v_scale;
         auto fill = [&](uint32_t table, int bits, float centre) {
             for (int e = warp; e < 1 << 2 * bits; e += kThreads / 32) {
                 const float lo = __shfl_sync(0xffffffffu, centre, e & ((1 << bits) - 1)), hi = __shfl_sync(0xffffffffu, centre, e >> bits);
@@ -906,8 +909,8 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     a.positions = p.positions, a.tiles = p.tiles, a.rows = p.rows, a.ctas = p.ctas;
     a.seq_start = cache->seq_start, a.lengths = lengths, a.mask = tree_mask;
     a.image_k = ctx->img_rot_k.data, a.image_s = ctx->img_qjl.data, a.image_v = ctx->img_rot_v.data;
-    a.unscale_k = kUmmaRestore * ctx->img_rot_k.unscale, a.unscale_s = kUmmaRestore * ctx->img_qjl.unscale, a.unscale_v = kUmmaRestore * ctx->img_rot_v.unscale;
-    a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v;
+    a.unscale_k = kUmmaRestore * ctx->img_rot_k.unscale, a.unscale_s = kUmmaRestore * ctx->img_qjl.unscale, a.unscale_v = kUmmaRestore * ctx->img_rot_v.unscale / (ctx->cen_v_scale * 0x1p-14f);
+    a.centers_k = ctx->centers_k, a.centers_v = ctx->centers_v, a.cen_v_scale = ctx->cen_v_scale * 0x1p-14f;
     a.q = q->data, a.qb = q->stride_b, a.qh = q->stride_h, a.qt = q->stride_t;
     a.out = const_cast<void *>(out->data), a.ob = out->stride_b, a.oh = out->stride_h, a.ot = out->stride_t;
     a.qop = reinterpret_cast<uint4 *>(ws + p.qop);
