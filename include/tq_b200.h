@@ -242,7 +242,7 @@ int32_t tq_cache_select_rows(tq_ctx *ctx, const tq_cache_desc *src, const tq_cac
  * device.  q / out [batch, q_heads, n_q, 128], k / v [batch, kv_heads, n_kv, 128], all fp16 or all bf16; outer strides
  * in elements, multiples of 8 (anything where the size is 1), data 16-byte aligned.  Query i sees the keys
  * [seq_start[b], i + n_kv - n_q] (causal; needs n_kv >= n_q) or [seq_start[b], n_kv).  seq_start: optional device int32
- * [batch], clamped to [0, n_kv].  A query that sees nothing gets zeros.  Keys and values before seq_start are not looked at: they may hold
+ * [batch], clamped to [0, n_kv].  A query that sees nothing gets zeros, one that sees logits of -inf alone NaN.  Keys and values before seq_start are not looked at: they may hold
  * anything.  Logits are scale * (q . k).
  *
  * tq_prompt_attn_packed: n_seqs sequences end to end, q / out [total, q_heads, 128], k / v [total, kv_heads, 128]

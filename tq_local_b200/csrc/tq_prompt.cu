@@ -72,6 +72,10 @@ __device__ __forceinline__ int2 sequence_of(const PromptArgs &a, int b) {
     return make_int2(first, min(min(a.cu_seqlens[b + 1], a.total) - first, a.n_q));
 }
 
+// What a row's sums are multiplied with.  A row that sees no key has zeros.  One whose logits are all -inf has no softmax: NaN (its sum is 0, or some 2^-125
+// where exponentials come from the polynomial).
+__device__ __forceinline__ float inverse_sum(float m, float l, bool sees) { return !sees ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l; }
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     tq_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -369,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else {
-            const bool any = l > 0.f || l != l;
-            const float inv = any ? 1.f / l : 0.f;
+            const bool any = limit > start;
+            const float inv = inverse_sum(m_ref, l, any);
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 uint32_t o[32] = {};
@@ -407,11 +411,11 @@ template <bool BF16> __global__ void __launch_bounds__(128) tq_prompt_join_kerne
     const int lane = threadIdx.x & 31, heads = a.kv_heads * a.group;
     if (r >= rows) return;
     const int head = (int)(r % heads), pos = (int)(r / heads % a.n_q), b = (int)(r / heads / a.n_q);
-    int t0 = 0;
+    int n_q = a.n_q, n_kv = a.n_kv, t0 = 0;
     if (a.cu_seqlens) {
         const int2 seq = sequence_of(a, b);
-        t0 = seq.x;
-        if (pos >= seq.y) return;
+        t0 = seq.x, n_q = n_kv = seq.y;
+        if (pos >= n_q) return;
     }
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + r * a.splits;
     float m = -INFINITY;
@@ -426,7 +430,9 @@ template <bool BF16> __global__ void __launch_bounds__(128) tq_prompt_join_kerne
         l += f * part.y;
         o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const int start = a.seq_start ? min(max(a.seq_start[b], 0), a.n_kv) : 0;  // (as in the kernel before)
+    const int limit = a.causal ? min(n_kv, pos + n_kv - n_q + 1) : n_kv;
+    const float inv = inverse_sum(m, l, limit > start);
     uint2 *dst = reinterpret_cast<uint2 *>(reinterpret_cast<uint8_t *>(a.out) + 2 * ((a.cu_seqlens ? 0 : b) * a.ob + head * a.oh + (int64_t)(t0 + pos) * a.ot)) + lane;
     *dst = make_uint2(pack16<BF16>(o.x * inv, o.y * inv), pack16<BF16>(o.z * inv, o.w * inv));
 }

@@ -61,7 +61,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     """``query`` [B, Hq, Sq, 128], ``key`` / ``value`` [B, Hkv, Skv, 128] (fp16 or bf16, any outer strides) -> [B, Hq, Sq, 128], a view of
     [B, Sq, Hq, 128].  Causal: query ``i`` sees the keys up to ``i + Skv - Sq`` (so ``Sq`` < ``Skv`` is a chunk behind
     ``Skv - Sq`` earlier tokens).  ``seq_start`` (int32 [B] on the device): entry ``b`` attends keys from there on, a
-    left-padded batch; a query that sees no key gets zeros.  ``scale`` defaults to 1/sqrt(128)."""
+    left-padded batch; a query that sees no key gets zeros, one whose logits are all -inf NaN.  ``scale`` defaults to 1/sqrt(128)."""
     _check(query, key, value, 4)
     (b, hq, n_q, _), (b_kv, hkv, n_kv, _) = query.shape, key.shape
     if b_kv != b or (causal and n_kv < n_q):
