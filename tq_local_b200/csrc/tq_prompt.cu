@@ -437,8 +437,9 @@ template <bool BF16> __global__ void __launch_bounds__(128) tq_prompt_join_kerne
     *dst = make_uint2(pack16<BF16>(o.x * inv, o.y * inv), pack16<BF16>(o.z * inv, o.w * inv));
 }
 
-bool aligned(const tq_dense_desc *d) {
-    return !(((uintptr_t)d->data | (uintptr_t)(2 * (d->stride_b | d->stride_h | d->stride_t))) & 15);
+bool aligned(const tq_dense_desc *d, int64_t batch, int heads, int64_t tokens) {  // (an axis of one element has no stride of its own)
+    const int64_t strides = (batch > 1 ? d->stride_b : 0) | (heads > 1 ? d->stride_h : 0) | (tokens > 1 ? d->stride_t : 0);
+    return !(((uintptr_t)d->data | (uintptr_t)(2 * strides)) & 15);
 }
 
 int sm_count() {
@@ -540,7 +541,11 @@ int32_t prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_den
     if (batch < 0 || n_q < 0 || n_kv < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads) return TQ_ERR_ARG;
     if (q_heads / kv_heads > TQ_MAX_PROMPT_GROUPS) return TQ_ERR_UNSUPPORTED;
     if (causal && n_kv < n_q) return TQ_ERR_ARG;
-    if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out)) return TQ_ERR_ARG;
+    const int64_t tokens_q = cu_seqlens ? total : n_q, tokens_kv = cu_seqlens ? total : n_kv;
+    const int maps_batch = cu_seqlens ? 1 : batch;
+    if (!aligned(q, maps_batch, q_heads, tokens_q) || !aligned(out, maps_batch, q_heads, tokens_q) || !aligned(k, maps_batch, kv_heads, tokens_kv) ||
+        !aligned(v, maps_batch, kv_heads, tokens_kv))
+        return TQ_ERR_ARG;
     if (((uintptr_t)seq_start | (uintptr_t)cu_seqlens) & 3 || (uintptr_t)workspace & 15) return TQ_ERR_ARG;
     const size_t need = tq_prompt_workspace_bytes(batch, q_heads, kv_heads, n_q, n_kv);
     if (workspace_bytes < need || (need && !workspace)) return TQ_ERR_WORKSPACE;
@@ -558,9 +563,8 @@ int32_t prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_den
         const size_t rows = (size_t)batch * n_q * q_heads * p.splits;
         a.part_o = static_cast<float *>(workspace), a.part_ml = a.part_o + rows * TQ_D;
     }
-    const int64_t tokens_q = cu_seqlens ? total : n_q, tokens_kv = cu_seqlens ? total : n_kv;
-    return q->dtype == TQ_DTYPE_BF16 ? launch<true>(q, k, v, tokens_q, tokens_kv, cu_seqlens ? 1 : batch, a, stream)
-                                     : launch<false>(q, k, v, tokens_q, tokens_kv, cu_seqlens ? 1 : batch, a, stream);
+    return q->dtype == TQ_DTYPE_BF16 ? launch<true>(q, k, v, tokens_q, tokens_kv, maps_batch, a, stream)
+                                     : launch<false>(q, k, v, tokens_q, tokens_kv, maps_batch, a, stream);
 }
 
 }  // namespace
