@@ -34,3 +34,25 @@ def test_strides_of_axes_with_one_element_are_not_looked_at():
     packed = lambda d, n=0, total=8, h=2: ffi.lib().tq_prompt_attn_packed(d, d, d, n, total, h, h, 4096, 8, 0.1, 1, None, 0, d, None)
     assert packed(desc(b=3)) == OK and packed(desc(h=5)) == ARG and packed(desc(t=7)) == ARG
     assert packed(desc(h=5), h=1) == OK and packed(desc(t=7), total=1) == OK
+
+
+def test_what_the_backend_takes():
+    """Everything that a call of the kernels would refuse goes to the model's own attention instead, the values' type, size and gradient among it."""
+    from types import SimpleNamespace
+
+    from tq_local_b200.runtime.prompt_attention import _takes
+
+    def tensor(*shape, dtype=torch.bfloat16, device="cuda", grad=False):
+        return SimpleNamespace(shape=torch.Size(shape), dtype=dtype, device=torch.device(device), requires_grad=grad)
+
+    q, kv = tensor(2, 8, 30, 128), tensor(2, 2, 30, 128)
+    takes = lambda q=q, k=kv, v=kv, mask=None, causal=True, dropout=0.0, **kw: _takes(q, k, v, mask, causal, dropout, kw)
+    with torch.enable_grad():
+        assert takes() and takes(q=tensor(2, 8, 3, 128)) and takes(sliding_window=None)
+        for name, shape in (("q", (2, 8, 30, 128)), ("k", (2, 2, 30, 128)), ("v", (2, 2, 30, 128))):
+            assert not takes(**{name: tensor(*shape, grad=True)}) and not takes(**{name: tensor(*shape, dtype=torch.float16)})
+            with torch.no_grad():
+                assert takes(**{name: tensor(*shape, grad=True)})
+    assert not takes(v=tensor(2, 2, 30, 64)) and not takes(k=tensor(2, 2, 30, 64)) and not takes(q=tensor(2, 8, 31, 128))
+    assert not takes(causal=False) and not takes(dropout=0.1) and not takes(sliding_window=4096) and not takes(softcap=30.0)
+    assert not takes(q=tensor(2, 8, 30, 128, device="cpu")) and not takes(q=tensor(2, 130, 30, 128))

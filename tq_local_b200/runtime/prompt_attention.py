@@ -116,13 +116,13 @@ def raise_on_status(device: torch.device, where: str) -> None:
                           "its outputs are not valid")
 
 
-def _takes(query, key, attention_mask, is_causal, dropout, kwargs) -> bool:
+def _takes(query, key, value, attention_mask, is_causal, dropout, kwargs) -> bool:
     """Whether the kernels compute what the model asks for here: causal attention of 16-bit tensors with 128 coordinates per head
     and at most left padding."""
     return (query.device.type == "cuda" and query.dtype in (torch.float16, torch.bfloat16) and key.dtype == query.dtype
-            and query.shape[-1] == 128 and key.shape[-1] == 128 and query.shape[2] <= key.shape[2] and is_causal and not dropout
+            and value.dtype == query.dtype and query.shape[-1] == 128 and key.shape[-1] == 128 and value.shape == key.shape and query.shape[2] <= key.shape[2] and is_causal and not dropout
             and query.shape[1] // key.shape[1] <= 64
-            and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad))
+            and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))
             and (attention_mask is None or attention_mask.dim() == 4)
             and not any(kwargs.get(name) is not None for name in ("sliding_window", "softcap", "s_aux", "position_bias")))
 
@@ -136,7 +136,7 @@ def turboquant_prompt_forward(module, query, key, value, attention_mask, dropout
     from tq_local_b200.runtime.packed_qmse_cache import leading_masked_tokens
 
     causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
-    if not _takes(query, key, attention_mask, causal, dropout, kwargs):
+    if not _takes(query, key, value, attention_mask, causal, dropout, kwargs):
         return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
     starts = None if attention_mask is None else leading_masked_tokens(attention_mask).expand(query.shape[0])
     return prompt_attention(query, key, value, scale=scaling, seq_start=starts).transpose(1, 2), None
