@@ -56,3 +56,26 @@ def test_what_the_backend_takes():
     assert not takes(v=tensor(2, 2, 30, 64)) and not takes(k=tensor(2, 2, 30, 64)) and not takes(q=tensor(2, 8, 31, 128))
     assert not takes(causal=False) and not takes(dropout=0.1) and not takes(sliding_window=4096) and not takes(softcap=30.0)
     assert not takes(q=tensor(2, 8, 30, 128, device="cpu")) and not takes(q=tensor(2, 130, 30, 128))
+
+
+def test_what_the_kernels_do_not_compute_is_the_models_own_attention():
+    """Not causal, a mask, dropout: as ``sdpa`` computes it."""
+    from types import SimpleNamespace
+
+    import torch.nn.functional as F
+
+    from tq_local_b200.runtime.prompt_attention import turboquant_prompt_forward
+
+    gen = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(2, h, 9, 16, generator=gen) for h in (4, 2, 2))
+    plain = lambda **kw: F.scaled_dot_product_attention(q, k.repeat_interleave(2, 1), v.repeat_interleave(2, 1), **kw).transpose(1, 2)
+    module = lambda causal: SimpleNamespace(is_causal=causal, num_key_value_groups=2, training=False)
+    for causal in (False, True):
+        out, weights = turboquant_prompt_forward(module(causal), q, k, v, None, scaling=0.3)
+        assert weights is None
+        torch.testing.assert_close(out, plain(is_causal=causal, scale=0.3))
+        torch.testing.assert_close(turboquant_prompt_forward(module(not causal), q, k, v, None, is_causal=causal)[0], plain(is_causal=causal))
+    mask = torch.rand(2, 1, 9, 9, generator=gen) < 0.7
+    mask[..., 0] = True
+    torch.testing.assert_close(turboquant_prompt_forward(module(True), q, k, v, mask)[0], plain(attn_mask=mask))
+    assert (turboquant_prompt_forward(module(False), q, k, v, None, dropout=1.0)[0] == 0).all()

@@ -131,13 +131,14 @@ def turboquant_prompt_forward(module, query, key, value, attention_mask, dropout
                               is_causal: bool | None = None, **kwargs):
     """HF attention function of the prompt pass, ``(module, query[B,Hq,Sq,D], key, value, mask, ...) -> (out[B,Sq,Hq,D], None)``.  The
     mask is that of a causal, at most left-padded batch (``generate`` switches here only for those); what the kernels do not compute
-    goes to ``F.scaled_dot_product_attention``."""
-    from tq_local_b200.runtime.attention import _sdpa_fallback
+    goes to the ``sdpa`` that the model runs otherwise, with all that the model hands down."""
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
     from tq_local_b200.runtime.packed_qmse_cache import leading_masked_tokens
 
     causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
     if not _takes(query, key, value, attention_mask, causal, dropout, kwargs):
-        return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
+        return ALL_ATTENTION_FUNCTIONS["sdpa"](module, query, key, value, attention_mask, dropout=dropout, scaling=scaling, is_causal=is_causal, **kwargs)
     starts = None if attention_mask is None else leading_masked_tokens(attention_mask).expand(query.shape[0])
     return prompt_attention(query, key, value, scale=scaling, seq_start=starts).transpose(1, 2), None
 
