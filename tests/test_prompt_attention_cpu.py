@@ -79,3 +79,24 @@ def test_what_the_kernels_do_not_compute_is_the_models_own_attention():
     mask[..., 0] = True
     torch.testing.assert_close(turboquant_prompt_forward(module(True), q, k, v, mask)[0], plain(attn_mask=mask))
     assert (turboquant_prompt_forward(module(False), q, k, v, None, dropout=1.0)[0] == 0).all()
+
+
+@pytest.mark.parametrize("before", [None, "sdpa"])
+@pytest.mark.parametrize("fails", [False, True])
+def test_a_models_implementation_is_put_back_as_it_was(before, fails):
+    from types import SimpleNamespace
+
+    from transformers import LlamaConfig
+
+    from tq_local_b200.runtime.generation import _prompt_kernels
+
+    model = SimpleNamespace(config=LlamaConfig(hidden_size=256, num_attention_heads=2, num_hidden_layers=1))
+    model.config._attn_implementation = before
+    try:
+        with _prompt_kernels(model, {"input_ids": torch.zeros(1, 4, dtype=torch.long)}, True):
+            assert model.config._attn_implementation == "turboquant_prompt"
+            if fails:
+                raise KeyError
+    except KeyError:
+        assert fails
+    assert model.config._attn_implementation == before

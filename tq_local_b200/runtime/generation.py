@@ -119,7 +119,7 @@ def _prompt_kernels(model, inputs, enabled: bool):
     try:
         yield
     finally:
-        config._attn_implementation = previous or "sdpa"
+        config._attn_implementation = previous
     if inputs["input_ids"].device.type == "cuda":
         raise_on_status(inputs["input_ids"].device, "prompt pass")
 
