@@ -38,3 +38,18 @@ def test_logits_of_minus_infinity(dtype, n, m):
         want = v[:, :, at].repeat_interleave(2, 1).unsqueeze(2).expand(3, 4, n - before, 128).double()
         # (the weight 1 and the sum 1 are exact, others are 0 or 2^-125)
         assert ((out[:, :, before:].double() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -25).all()
+
+
+def test_the_status_waits_for_every_stream():
+    """What a kernel on a stream of its own reports is not missed."""
+    from tq_local_b200.runtime.prompt_attention import prompt_attention, raise_on_status
+
+    q = torch.zeros(1, 2, 8, 128, device="cuda", dtype=BF16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # some 50 ms
+        prompt_attention(q, q, q)
+    assert not side.query()
+    raise_on_status(q.device, "test")
+    assert side.query()

@@ -596,6 +596,7 @@ extern "C" int32_t tq_prompt_attn_packed(const tq_dense_desc *q, const tq_dense_
 extern "C" int32_t tq_prompt_status(int32_t *status_out) {
     if (!status_out) return TQ_ERR_ARG;
     int v = 0;
+    TQ_CUDA_CHECK(cudaDeviceSynchronize());  // (the copy alone does not wait for streams that do not block with the default one)
     TQ_CUDA_CHECK(cudaMemcpyFromSymbol(&v, g_prompt_status, sizeof(v)));
     *status_out = v;
     return TQ_OK;
