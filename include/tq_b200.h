@@ -250,7 +250,7 @@ int32_t tq_cache_select_rows(tq_ctx *ctx, const tq_cache_desc *src, const tq_cac
  * not above total), of at most max_seqlen tokens; tokens beyond that, and those behind the last sequence, are left as
  * they were in out.
  * tq_prompt_status: synchronises with the current device; 0; 1 when a kernel's bounded wait ran out, 2 when its
- * shared memory was not laid out as it needs (sticky). */
+ * shared memory was not laid out as it needs.  One word per device, which stays until tq_prompt_status_clear. */
 size_t tq_prompt_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv);
 int32_t tq_prompt_attn(const tq_dense_desc *q, const tq_dense_desc *k, const tq_dense_desc *v, int32_t batch,
                        int32_t q_heads, int32_t kv_heads, int32_t n_q, int32_t n_kv, const int32_t *seq_start, float scale,
@@ -260,6 +260,7 @@ int32_t tq_prompt_attn_packed(const tq_dense_desc *q, const tq_dense_desc *k, co
                               int32_t max_seqlen, float scale, int32_t causal, void *workspace, size_t workspace_bytes,
                               const tq_dense_desc *out, tq_stream stream);
 int32_t tq_prompt_status(int32_t *status_out);
+int32_t tq_prompt_status_clear(void);
 
 /* ---- KV-head sharding over the GPUs of one box (no counterpart in the reference, which is
  * single-GPU).  Rank r serves kv_heads / world KV heads and their query heads; the only exchange

@@ -53,3 +53,13 @@ def test_the_status_waits_for_every_stream():
     assert not side.query()
     raise_on_status(q.device, "test")
     assert side.query()
+
+
+def test_the_status_can_be_cleared():
+    import ctypes as C
+
+    from tq_local_b200.runtime import ffi
+
+    word = C.c_int32(-1)
+    assert ffi.lib().tq_prompt_status_clear() == 0
+    assert ffi.lib().tq_prompt_status(C.byref(word)) == 0 and word.value == 0

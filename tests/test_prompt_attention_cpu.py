@@ -100,3 +100,30 @@ def test_a_models_implementation_is_put_back_as_it_was(before, fails):
     except KeyError:
         assert fails
     assert model.config._attn_implementation == before
+
+
+def test_a_lost_wait_is_reported_once(monkeypatch):
+    """The device's word stays until it is cleared, so that it must be once it has been reported: later calls are not at fault."""
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+
+    from tq_local_b200.runtime import ffi, prompt_attention
+
+    word = {"now": 0}
+
+    def status(out):
+        out._obj.value = word["now"]
+        return 0
+
+    def clear():
+        word["now"] = 0
+        return 0
+
+    monkeypatch.setattr(ffi, "lib", lambda: SimpleNamespace(tq_prompt_status=status, tq_prompt_status_clear=clear))
+    monkeypatch.setattr(torch.cuda, "device", lambda device: nullcontext())
+    prompt_attention.raise_on_status("cuda:0", "here")
+    for lost in (1, 2):
+        word["now"] = lost
+        with pytest.raises(ffi.TQError, match=f"here.*status {lost}"):
+            prompt_attention.raise_on_status("cuda:0", "here")
+        prompt_attention.raise_on_status("cuda:0", "here")

@@ -601,3 +601,9 @@ extern "C" int32_t tq_prompt_status(int32_t *status_out) {
     *status_out = v;
     return TQ_OK;
 }
+
+extern "C" int32_t tq_prompt_status_clear(void) {
+    const int v = 0;
+    TQ_CUDA_CHECK(cudaMemcpyToSymbol(g_prompt_status, &v, sizeof(v)));
+    return TQ_OK;
+}

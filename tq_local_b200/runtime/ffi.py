@@ -27,7 +27,7 @@ EXPORTS = (
     "tq_decode_attn_gather", "tq_gather_wait", "tq_decode_step_host_gather", "tq_set_wait_limit_ms", "tq_decode_attn_f32out",
     "tq_parts_exchange_bytes", "tq_decode_attn_parts", "tq_decode_parts_finish",
     "tq_tree_workspace_bytes", "tq_tree_attn", "tq_cache_keep_tokens", "tq_cache_select_rows",
-    "tq_prompt_workspace_bytes", "tq_prompt_attn", "tq_prompt_attn_packed", "tq_prompt_status",
+    "tq_prompt_workspace_bytes", "tq_prompt_attn", "tq_prompt_attn_packed", "tq_prompt_status", "tq_prompt_status_clear",
 )
 
 _ERRORS = {-1: "bad argument", -2: "unsupported shape or mode", -3: "CUDA error", -4: "workspace too small"}
@@ -168,8 +168,9 @@ def lib() -> C.CDLL:
     L.tq_prompt_attn_packed.argtypes = [dense, dense, dense] + [C.c_int32] * 4 + [C.c_void_p, C.c_int32, C.c_float, C.c_int32,
                                                                                  C.c_void_p, C.c_size_t, dense, C.c_void_p]
     L.tq_prompt_status.argtypes = [C.POINTER(C.c_int32)]
+    L.tq_prompt_status_clear.argtypes = []
     for name in ("tq_tree_attn", "tq_cache_keep_tokens", "tq_cache_select_rows", "tq_prompt_attn", "tq_prompt_attn_packed",
-                 "tq_prompt_status"):
+                 "tq_prompt_status", "tq_prompt_status_clear"):
         getattr(L, name).restype = C.c_int32
     L.tq_set_wait_limit_ms.argtypes = [C.c_void_p, C.c_int32]
     L.tq_set_wait_limit_ms.restype = C.c_int32

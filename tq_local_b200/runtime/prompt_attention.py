@@ -107,10 +107,13 @@ def prompt_attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch
 
 
 def raise_on_status(device: torch.device, where: str) -> None:
-    """Raise :class:`TQError` when a prompt kernel of this device has given up waiting (synchronises with the device)."""
+    """Raise :class:`TQError` when a prompt kernel of this device has given up waiting (synchronises with the device).  What is reported is
+    cleared: later calls are judged by themselves."""
     v = C.c_int32()
     with torch.cuda.device(device):
         ffi.check(ffi.lib().tq_prompt_status(C.byref(v)), "tq_prompt_status")
+        if v.value:
+            ffi.check(ffi.lib().tq_prompt_status_clear(), "tq_prompt_status_clear")
     if v.value:
         raise ffi.TQError(f"{where}: a prompt attention kernel gave up (status {v.value}: 1 a wait ran out, 2 its shared memory did not fit); "
                           "its outputs are not valid")
