@@ -589,7 +589,7 @@ class PackedMSELayer(CacheLayerMixin):
     def bind_tree(self, tree_mask: torch.Tensor | None, lengths: torch.Tensor | None = None) -> None:
         """The next model steps are of drafted tokens: a step's T tokens are appended as usual and ``attend`` lets each
         see its history and what ``tree_mask`` says of the others (see ``PackedStore.tree_attn``) instead of going
-        through them one at a time.  ``unbind_tree`` ends this."""
+        through them one at a time.  Masks and lengths per row follow their rows when those move.  ``unbind_tree`` ends this."""
         self._plain_store("bind_tree")
         if not self.quantize_decode or self._static_pos is not None:
             raise RuntimeError("drafted tokens are packed ones: quantize_decode=True, outside a static decode")
@@ -617,19 +617,27 @@ class PackedMSELayer(CacheLayerMixin):
         if self._static_pos is not None:
             raise RuntimeError(f"{what} inside a static decode")
 
+    def _take_rows(self, index: torch.Tensor) -> None:
+        """What a layer holds per row beside its store: dense tokens, and the mask and the lengths of a bound tree."""
+        self._dense_k.take_rows(index), self._dense_v.take_rows(index)
+        if self._tree is not None:
+            take = lambda t: None if t is None else t.index_select(0, index.to(t.device))
+            mask, lengths = self._tree
+            self._tree = (mask if mask is not None and mask.dim() == 1 else take(mask), take(lengths))  # (one mask for all rows stays)
+
     def reorder_cache(self, beam_idx: torch.Tensor) -> None:
         """Row ``b`` of the cache becomes what row ``beam_idx[b]`` was."""
         self._before_rows_move("reorder_cache")
         if self.store is not None:
             self.store.select_rows(beam_idx.to(self.device))
-        self._dense_k.take_rows(beam_idx), self._dense_v.take_rows(beam_idx)
+        self._take_rows(beam_idx)
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         """The cache of a batch of ``len(indices)`` rows: row ``i`` is what row ``indices[i]`` was."""
         self._before_rows_move("batch_select_indices")
         if self.store is not None:
             self.store = self.store.take_rows(indices.to(self.device))
-        self._dense_k.take_rows(indices), self._dense_v.take_rows(indices)
+        self._take_rows(indices)
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         """Every row ``repeats`` times, side by side."""
