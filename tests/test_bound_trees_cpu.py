@@ -32,3 +32,20 @@ def test_masks_and_lengths_follow_their_rows(rows, dtype):
     layer.unbind_tree()
     layer.reorder_cache(index)
     assert layer._tree is None
+
+
+def test_a_static_decode_does_not_begin_under_a_bound_tree():
+    """Its steps would attend every row up to the longest and none of the mask."""
+    from types import SimpleNamespace
+
+    layer = layer_of(None, torch.tensor([5], dtype=torch.int32))
+    layer.store = SimpleNamespace(length=5, reserve=lambda n: None)
+    pos = torch.zeros((), dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="unbind_tree"):
+        layer.begin_static_decode(pos, 4)
+    assert layer._static_pos is None
+    layer.unbind_tree()
+    layer.begin_static_decode(pos, 4)
+    assert layer._static_pos is pos
+    with pytest.raises(RuntimeError):
+        layer.bind_tree(None)

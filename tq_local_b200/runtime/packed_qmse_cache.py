@@ -383,6 +383,8 @@ class PackedMSELayer(CacheLayerMixin):
         graph.  ``end_static_decode`` returns to the normal bookkeeping."""
         if self.shard.world_size > 1 and gather is None:
             raise RuntimeError("a sharded layer needs a PeerGather(device_sequence=True) for static decode")
+        if self._tree is not None:
+            raise RuntimeError("a static decode step does not look at a bound tree: unbind_tree first")
         self.store.reserve(self.store.length + int(max_new_tokens))
         self._static_pos = pos
         self._static_gather = gather if self.shard.world_size > 1 else None
