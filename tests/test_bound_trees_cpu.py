@@ -49,3 +49,19 @@ def test_a_static_decode_does_not_begin_under_a_bound_tree():
     assert layer._static_pos is pos
     with pytest.raises(RuntimeError):
         layer.bind_tree(None)
+
+
+def test_layers_of_float32_models_are_refused_before_a_step_has_changed_them():
+    from types import SimpleNamespace
+
+    layer = layer_of(None, None)
+    layer.unbind_tree()
+    layer.store = SimpleNamespace(length=5)
+    layer.dtype = torch.float32
+    with pytest.raises(NotImplementedError, match="float32"):
+        layer.bind_tree(None)
+    assert layer._tree is None
+    for dtype in (torch.float16, torch.bfloat16):
+        layer.dtype = dtype
+        layer.bind_tree(None)
+        assert layer._tree == (None, None)

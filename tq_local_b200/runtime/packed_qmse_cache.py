@@ -595,6 +595,8 @@ class PackedMSELayer(CacheLayerMixin):
         self._plain_store("bind_tree")
         if not self.quantize_decode or self._static_pos is not None:
             raise RuntimeError("drafted tokens are packed ones: quantize_decode=True, outside a static decode")
+        if self.dtype not in (torch.float16, torch.bfloat16):
+            raise NotImplementedError(f"drafted tokens are attended in float16 or bfloat16; this layer holds {self.dtype}")
         self._tree = (tree_mask, lengths)
 
     def unbind_tree(self) -> None:
