@@ -66,3 +66,13 @@ def test_waits_for_tensor_memory_name_the_registers_that_arrive():
                 found += 1
                 assert "tcgen05.ld." in statement or '"+r"' in statement, (name, statement)
     assert found == 2
+
+
+def test_every_shared_piece_has_a_caller():
+    """Functions of the headers, each named at least once outside its own definition."""
+    files = {name: re.sub(r"//[^\n]*", "", source(name)) for name in os.listdir(CSRC) if name.endswith((".cu", ".cuh"))}
+    for name in ("tq_attn_tc.cuh", "tq_umma.cuh", "tq_bulk.cuh"):
+        for function in set(re.findall(r"__forceinline__ [\w:]+ \*?(\w+)\(", files[name])):
+            uses = sum(len(re.findall(rf"\b{function}\b", text)) for text in files.values())
+            defined = len(re.findall(rf"__forceinline__ [\w:]+ \*?{function}\(", files[name]))
+            assert uses > defined, (name, function)

@@ -1,5 +1,5 @@
-// Pieces shared by the tcgen05 attention kernels: products with both operands in shared memory or A in TMEM, TMEM moves of 32 columns,
-// tensor-map copies, and the exponentials of a row.
+// Pieces of the tcgen05 attention kernels: single products with both operands in shared memory, O += P V with the weights in TMEM, TMEM moves of 16
+// and 32 columns, arrivals of a warp, and the exponentials of a row.
 #pragma once
 
 #include "tq_umma.cuh"
@@ -19,15 +19,6 @@ __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64
         : "memory");
 }
 
-// D[128 x 128] = A[128 x 128] * B^T, both row-major images of two 64-wide slabs (see umma_operand_offset).
-__device__ __forceinline__ void attn_scores(uint32_t d, uint32_t a_addr, uint32_t b_addr, uint32_t instr, uint32_t accumulate = 0) {
-    const uint64_t a = umma_desc<false>(a_addr), b = umma_desc<false>(b_addr);
-#pragma unroll
-    for (uint32_t s = 0; s < 8; ++s) {
-        const uint32_t step = ((s >> 2) * kUmmaSlabBytes + (s & 3) * 32) >> 4;
-        umma_ss(d, a + step, b + step, instr, accumulate | (s > 0));
-    }
-}
 // D[128 x 128] (+)= P[128 x 128] * V, P as packed 16-bit pairs in TMEM, V a row-major image (rows are tokens).
 __device__ __forceinline__ void attn_values(uint32_t d, uint32_t p, uint32_t v_addr, uint32_t instr, uint32_t accumulate) {
     const uint64_t b = umma_desc<true>(v_addr);

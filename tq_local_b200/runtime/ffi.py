@@ -16,7 +16,6 @@ LIB_PATH = os.environ.get("TQ_B200_LIBRARY") or os.path.join(_PKG, "libtq_b200.s
 
 TQ_DTYPE_F32, TQ_DTYPE_F16, TQ_DTYPE_BF16 = 0, 1, 2
 TQ_MAX_GROUPS = 8
-TQ_MAX_TREE = 64
 
 EXPORTS = (
     "tq_abi_version", "tq_last_cuda_error", "tq_ctx_create", "tq_ctx_destroy", "tq_pack",
