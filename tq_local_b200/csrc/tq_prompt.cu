@@ -455,6 +455,8 @@ int sm_count() {
 // with one tile and 2.3 with two (whose products and exponentials go on beside each other), starting and ending one 4, joining pieces 6 (512 queries
 // behind 16384 keys, 32 / 8 heads: 197 us with one tile and one piece, 141 as chosen here: two tiles, two pieces).  Under a causal mask a tile sees the keys before
 // the queries and half of theirs on average.
+// At most 32 pieces: one query behind 32768 keys, 4 / 1 heads, 31.1 us with 16, 23.8 with 32, 24.7 with 64 (behind 131072, 8 / 2 heads, 98, 59 and 45).  Of two
+// blocks at least: one query behind 2048 keys, 32 / 8 heads, 12.5 us with one, 12.0 with two, 13.5 with four, behind 1024 11.0, 11.0 and 16.2.
 struct Plan {
     int positions, tiles_per_cta, n_items, splits;
 };
