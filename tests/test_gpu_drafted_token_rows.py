@@ -158,3 +158,61 @@ def test_the_largest_values(bits, qjl):
     store.v_norms[:, :, ::3] = 65504.0
     q = queries(1, 8, 5, BF16)
     check(store.tree_attn(q), *expected(store, q, 195))
+
+
+def words(mask):
+    """bool [..., T, T] -> int64 [..., T]"""
+    t = mask.shape[-1]
+    return (mask.long() << torch.arange(t, device=mask.device)).sum(-1)
+
+
+def random_tree(b, t, seed):
+    gen = torch.Generator().manual_seed(seed)
+    mask = torch.zeros(b, t, t, dtype=torch.bool)
+    for r in range(b):
+        for i in range(t):
+            up = int(torch.randint(-1, i, (1,), generator=gen)) if i else -1
+            if up >= 0:
+                mask[r, i] = mask[r, up]
+            mask[r, i, i] = True
+    return mask.cuda()
+
+
+@pytest.mark.parametrize("bits,qjl", [(4, True), (3, False), (2, True)])
+@pytest.mark.parametrize("t,dtype", [(1, F16), (12, BF16)])
+def test_rows_of_histories_of_different_lengths(bits, qjl, t, dtype):
+    """Rows that see one token lie beside rows that see hundreds, whose outputs are many times smaller."""
+    lengths = torch.tensor([700, 0, 1, 127, 128, 129, 512, 699, -5, 10_000], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([699, 0, 1, 5, 128, 64, 130, 700, 3, -1], dtype=torch.int32, device="cuda")
+    b = len(lengths)
+    store = store_of(bits, qjl, normal(b, 2, 700 + t, seed=t).to(BF16), normal(b, 2, 700 + t, seed=t + 1).to(BF16), capacity=900)
+    q, mask = queries(b, 8, t, dtype), random_tree(b, t, 5)
+    check(store.tree_attn(q, words(mask), lengths=lengths), *expected(store, q, 700, mask, lengths))
+    store.set_seq_start(starts)
+    check(store.tree_attn(q, words(mask), lengths=lengths), *expected(store, q, 700, mask, lengths, starts))
+    check(store.tree_attn(q, lengths=lengths), *expected(store, q, 700, None, lengths, starts))
+
+
+@pytest.mark.parametrize("bits,qjl", [(4, True), (2, False)])
+@pytest.mark.parametrize("b,hq,hkv,n,t,dtype", [(3, 16, 8, 4500, 3, F16), (2, 28, 4, 3001, 64, BF16), (40, 16, 8, 200, 1, F16), (1, 4, 2, 30_000, 40, F16),
+                                                (1, 8, 1, 5000, 200, BF16)])
+def test_rows_that_are_joined_from_pieces(bits, qjl, b, hq, hkv, n, t, dtype):
+    store = store_of(bits, qjl, normal(b, hkv, n + t, seed=b).to(BF16), normal(b, hkv, n + t, seed=b + 1).to(BF16))
+    lengths = torch.randint(0, n + 1, (b,), generator=torch.Generator().manual_seed(b), dtype=torch.int32).cuda()
+    q, mask = queries(b, hq, t, dtype), random_tree(b, t, 9) if t <= 64 else None
+    check(store.tree_attn(q, None if mask is None else words(mask), lengths=lengths), *expected(store, q, n, mask, lengths))
+    assert store.codec.device_status() == 0
+
+
+@pytest.mark.parametrize("bits,qjl", [(4, True), (3, False), (2, True)])
+def test_rows_over_norms_of_all_sizes(bits, qjl):
+    """Keys and values from 2^-20 to 2^10 of their usual length, zeros among them; each head's values of one size of their own."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    sizes = lambda lo, hi, *s: torch.exp2(torch.randint(lo, hi, (*s, 1), device="cuda", generator=gen).float())
+    k = normal(3, 4, 400, seed=3, spread=0.0) * sizes(-20, 3, 3, 4, 400)
+    v = normal(3, 4, 400, seed=4, spread=0.0) * sizes(-3, 3, 3, 4, 400) * sizes(-9, 8, 3, 4, 1)
+    k[:, :, ::17] = 0
+    v[:, :, 5::19] = 0
+    store = store_of(bits, qjl, k, v)
+    q = queries(3, 16, 9, BF16)
+    check(store.tree_attn(q), *expected(store, q, 391))
