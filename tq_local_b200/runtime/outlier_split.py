@@ -229,7 +229,7 @@ class SplitStore:
                 gs.reserve(capacity, self.length)
             self.capacity = capacity
 
-    def set_seq_start(self, seq_start: torch.Tensor | None) -> None:
+    def set_seq_start(self, seq_start: torch.Tensor | None, own: bool = False) -> None:
         self._seq_start = seq_start
 
     def storage_bytes(self) -> int:

@@ -527,7 +527,7 @@ class PackedMSELayer(CacheLayerMixin):
             return
         if mask is not None and self.seq_parts > 1:
             raise NotImplementedError("padded batches are not available when several ranks share a KV head")
-        self.store.set_seq_start(None if mask is None else leading_masked_tokens(mask))
+        self.store.set_seq_start(None if mask is None else leading_masked_tokens(mask), own=True)
         self._mask_bound = (mask is not None) if lock is None else bool(lock)
 
     def attend(self, query_states: torch.Tensor, attention_mask: torch.Tensor | None = None) -> torch.Tensor:
@@ -541,7 +541,7 @@ class PackedMSELayer(CacheLayerMixin):
             raise RuntimeError("attend() needs a packed (non-dense) layer")
         if not self._mask_bound and self._static_pos is None:  # (a recorded step keeps the offsets it was given)
             if attention_mask is not None:
-                self.store.set_seq_start(leading_masked_tokens(attention_mask))
+                self.store.set_seq_start(leading_masked_tokens(attention_mask), own=True)
             elif self.store._seq_start is not None:
                 self.store.set_seq_start(None)
         if self._static_pos is not None:
@@ -676,7 +676,7 @@ class PackedMSELayer(CacheLayerMixin):
         if self.store is None or self._force_dense:
             raise RuntimeError("attend_with_new_tokens() needs a packed (non-dense) layer")
         if attention_mask is not None and not self._mask_bound:
-            self.store.set_seq_start(leading_masked_tokens(attention_mask))
+            self.store.set_seq_start(leading_masked_tokens(attention_mask), own=True)
         q_local = self.shard.local_q(query_states, self._kv_heads_total)
         tail_k, tail_v = self.shard.local_kv(new_key), self.shard.local_kv(new_value)
         if self._dense_k.length:

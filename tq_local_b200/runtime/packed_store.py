@@ -36,6 +36,7 @@ class PackedStore:
         self.batch, self.kv_heads = int(batch), int(kv_heads)
         self.length = 0
         self._seq_start: torch.Tensor | None = None  # see set_seq_start
+        self._own_starts = False  # nobody else holds it: it may be written
         self._alloc(max(8, _round_up(int(capacity), 8)))
         self._workspace: torch.Tensor | None = None
         self._step_plan = None
@@ -68,15 +69,16 @@ class PackedStore:
         self._desc_ref = C.byref(self._desc)
         self._step_plan = None
 
-    def set_seq_start(self, seq_start: torch.Tensor | None) -> None:
+    def set_seq_start(self, seq_start: torch.Tensor | None, own: bool = False) -> None:
         """Per-row first attended token (int32 [batch] on the cache's device): the decode calls then
         attend tokens ``[seq_start[b], length)`` of batch entry ``b`` - a left-padded batch.  ``None``
-        (the default) attends every row from token 0."""
+        (the default) attends every row from token 0.  ``own``: the caller gives the tensor up, and
+        ``select_rows`` writes the rows' new offsets to it."""
         if seq_start is not None:
             if seq_start.dtype != torch.int32 or seq_start.device != self.codec.device or \
                     tuple(seq_start.shape) != (self.batch,) or not seq_start.is_contiguous():
                 raise ValueError(f"seq_start must be a contiguous int32 tensor [{self.batch}] on {self.codec.device}")
-        self._seq_start = seq_start
+        self._seq_start, self._own_starts = seq_start, own
         self._desc.seq_start = seq_start.data_ptr() if seq_start is not None else None
 
     def streams(self) -> list[torch.Tensor]:
@@ -489,18 +491,22 @@ class PackedStore:
     def select_rows(self, index: torch.Tensor, lo: int = 0, hi: int | None = None) -> None:
         """Row ``b`` becomes what row ``index[b]`` was (int32 or int64 [B] on the device): a beam search's reordering.  Only tokens
         ``[lo, hi)`` are moved (default: all packed ones), for rows that share what lies before ``lo``; per-row offsets
-        (``set_seq_start``) go along.  A row whose index is out of range stays as it is and is reported (device status 7)."""
+        (``set_seq_start``) go along: where the cache owns their tensor in place, so that what was recorded with it attends the right tokens
+        afterwards; a tensor that the caller has kept is left alone and replaced by one that the cache owns, and what was recorded before that has
+        to be recorded again.  A row whose index is out of range stays as it is and is reported (device status 7)."""
         index = self._index(index)
         hi = self.length if hi is None else int(hi)
         if index.numel() != self.batch or not 0 <= int(lo) <= hi <= self.length:
             raise ValueError(f"select_rows takes {self.batch} rows and tokens within [0, {self.length}), got {index.numel()} and [{lo}, {hi})")
-        if self._seq_start is not None and torch.cuda.is_current_stream_capturing():
+        if self._seq_start is not None and not self._own_starts and torch.cuda.is_current_stream_capturing():
             raise ffi.TQError("select_rows gives a left-padded cache new offsets: a replayed graph would start from the old ones")
         starts = None if self._seq_start is None else torch.empty_like(self._seq_start)
         ffi.launch("tq_cache_select_rows", self.codec.device, (
             self.codec.handle, self._desc_ref, self._desc_ref, index.data_ptr(), int(lo), hi, None if starts is None else starts.data_ptr()))
-        if starts is not None:
-            self.set_seq_start(starts)
+        if starts is not None and self._own_starts:
+            self._seq_start.copy_(starts)
+        elif starts is not None:
+            self.set_seq_start(starts, own=True)
 
     def take_rows(self, index: torch.Tensor, capacity: int | None = None) -> "PackedStore":
         """A new store whose row ``i`` holds what row ``index[i]`` of this one holds: a batch that forks, grows or shrinks.  Rows
@@ -515,7 +521,7 @@ class PackedStore:
         ffi.launch("tq_cache_select_rows", self.codec.device, (
             self.codec.handle, self._desc_ref, other._desc_ref, index.data_ptr(), 0, self.length, None if starts is None else starts.data_ptr()))
         other.length = self.length
-        other.set_seq_start(starts)
+        other.set_seq_start(starts, own=True)
         return other
 
     def dequant(self, which: str, lo: int = 0, hi: int | None = None,
