@@ -191,6 +191,7 @@ def test_rows_of_histories_of_different_lengths(bits, qjl, t, dtype):
     store.set_seq_start(starts)
     check(store.tree_attn(q, words(mask), lengths=lengths), *expected(store, q, 700, mask, lengths, starts))
     check(store.tree_attn(q, lengths=lengths), *expected(store, q, 700, None, lengths, starts))
+    assert store.codec.device_status() == 0
 
 
 @pytest.mark.parametrize("bits,qjl", [(4, True), (2, False)])
@@ -216,3 +217,20 @@ def test_rows_over_norms_of_all_sizes(bits, qjl):
     store = store_of(bits, qjl, k, v)
     q = queries(3, 16, 9, BF16)
     check(store.tree_attn(q), *expected(store, q, 391))
+
+
+def test_a_sample_on_the_bounds_checked_build():
+    """Every bulk copy and every stored piece lies inside the cache's rows and the workspace: the cases assert a clean status word
+    themselves."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.join(root, "tq_local_b200", "libtq_b200_checked.so")
+    assert os.path.isfile(lib), "build it with `python -m tq_local_b200.build --checked`"
+    out = subprocess.run([sys.executable, "-m", "pytest", os.path.abspath(__file__), "-m", "gpu", "-x", "-q", "-k",
+                          "different_lengths or joined or (block_to_block and 40)"], capture_output=True, text=True, timeout=600,
+                         env=dict(os.environ, TQ_B200_LIBRARY=lib), cwd=root)
+    assert out.returncode == 0, out.stdout[-3000:] + out.stderr[-2000:]
+    assert " passed" in out.stdout and "failed" not in out.stdout

@@ -5,9 +5,9 @@ under ``csrc/`` into ``tq_local_b200/libtq_b200.so``.  Nothing is JIT-compiled a
 import time; the package fails loudly when the library is missing.
 
 ``--checked`` (``build_library(checked=True)``) builds ``libtq_b200_checked.so`` from the same
-sources with ``-DTQ_DEBUG_BOUNDS``: the decode kernel then checks every bulk-copy request and
-every partial it stores against the cache's and the workspace's extents, records a violation in
-the device status word (6) and drops the access instead of making it.  Point the environment
+sources with ``-DTQ_DEBUG_BOUNDS``: the decode kernel and that of drafted tokens then check every bulk-copy request and
+every partial they store against the cache's and the workspace's extents, record a violation in
+the device status word (6) and drop the access instead of making it.  Point the environment
 variable ``TQ_B200_LIBRARY`` at it to run anything (the test suite included) on the checked build;
 ``compute-sanitizer`` is not available where this library is developed, this build stands in.
 """

@@ -43,6 +43,7 @@ struct TreeArgs {
     const uint8_t *k_codes, *k_signs, *v_codes;
     const uint16_t *k_norms, *k_rnorms, *v_norms;
     int64_t cache_sb, cache_sh;
+    int capacity;  // tokens of a row (looked at by the bounds-checked build)
     int batch, kv_heads, group, nodes, tree_start;
     int positions, tiles, rows;  // nodes of a tile, tiles of a (batch entry, KV head), rows of a tile that hold something
     const int *seq_start, *lengths;
@@ -436,6 +437,19 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
                         if (n >= kRingSlots) wait(bar_read + 8 * slot, (n / kRingSlots & 1) ^ 1);
                         const uint32_t bar = bar_raw + 8 * slot, dst = base + L::kRing + slot * L::kSlot;
                         const int n0 = max(min(kBlock, tree - at), 0), n1 = max(min(kBlock, tree_end - at) - n0, 0);
+#ifdef TQ_DEBUG_BOUNDS
+                        // Both runs of tokens lie inside their row and the slot inside shared memory; what does not is recorded (status 6) and left out.
+                        uint32_t dyn_size;
+                        asm("mov.u32 %0, %%dynamic_smem_size;\n" : "=r"(dyn_size));
+                        const int t0 = g.e.first + at, t1 = (a.tree_start & ~7) + at + n0 - tree;
+                        if (g.b < 0 || g.b >= a.batch || g.h < 0 || g.h >= a.kv_heads || n0 + n1 <= 0 || n0 + n1 > kBlock || ((n0 | n1) & 7) ||
+                            (n0 && (t0 < 0 || t0 + n0 > a.capacity)) || (n1 && (t1 < 0 || t1 + n1 > a.capacity)) ||
+                            dst + L::kSlot > smem_u32(smem_raw) + dyn_size) {
+                            atomicExch(a.error_flag, 6);
+                            mbar_arrive_one(bar);
+                            continue;
+                        }
+#endif
                         mbar_expect_tx(bar, (n0 + n1) * L::kTokenBytes);
                         auto run = [&](int to, int64_t t, int count) {
                             tma_load_1d(dst + L::kRawK + to * 16 * KB, a.k_codes + t * 16 * KB, count * 16 * KB, bar);
@@ -656,14 +670,20 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             __syncwarp();
             umma_fence_after();
             const int64_t r = (g.tile + blockIdx.x) * a.rows + row;
-            if (live && half == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * r) = make_float2(m_ref, l);
+#ifdef TQ_DEBUG_BOUNDS
+            const bool known = r >= 0 && r < ((int64_t)a.batch * a.kv_heads * a.tiles + a.ctas) * a.rows;  // a piece that the workspace has
+            if (live && !known) atomicExch(a.error_flag, 6);
+#else
+            constexpr bool known = true;
+#endif
+            if (known && live && half == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * r) = make_float2(m_ref, l);
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
                 uint32_t o[32];
                 __syncwarp();
                 tmem_ld32(t_mine + 32 * i, o);
                 tmem_ld_wait(o);
-                if (live)
+                if (known && live)
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         a.part_o[((g.tile + blockIdx.x) * 32 + 16 * half + 8 * i + e) * a.rows + row] =
@@ -903,7 +923,7 @@ extern "C" int32_t tq_tree_attn(tq_ctx *ctx, const tq_dense_desc *q, int32_t q_h
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     TreeArgs a = {};
     a.k_codes = cache->k_codes, a.k_norms = cache->k_norms, a.k_signs = cache->k_signs, a.k_rnorms = cache->k_rnorms;
-    a.v_codes = cache->v_codes, a.v_norms = cache->v_norms, a.cache_sb = cache->stride_b, a.cache_sh = cache->stride_h;
+    a.v_codes = cache->v_codes, a.v_norms = cache->v_norms, a.cache_sb = cache->stride_b, a.cache_sh = cache->stride_h, a.capacity = cache->capacity;
     a.batch = cache->batch, a.kv_heads = cache->kv_heads, a.group = q_heads / cache->kv_heads, a.nodes = n_nodes, a.tree_start = tree_start;
     a.positions = p.positions, a.tiles = p.tiles, a.rows = p.rows, a.ctas = p.ctas;
     a.seq_start = cache->seq_start, a.lengths = lengths, a.mask = tree_mask;
