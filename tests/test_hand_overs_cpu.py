@@ -76,3 +76,15 @@ def test_every_shared_piece_has_a_caller():
             uses = sum(len(re.findall(rf"\b{function}\b", text)) for text in files.values())
             defined = len(re.findall(rf"__forceinline__ [\w:]+ \*?{function}\(", files[name]))
             assert uses > defined, (name, function)
+
+
+def test_copies_and_products_end_before_their_cta():
+    """A thread whose wait ran out waits for nothing more, but before the CTA ends what it set going is waited for: a copy that lands later would land
+    in another CTA's shared memory."""
+    for name, copies in (("tq_prompt.cu", ("mbar_wait(bar_full", "mbar_wait(bar_q")), ("tq_tree.cu", ("mbar_wait(bar_raw",))):
+        text = source(name)
+        end = text[text.index("if (__syncthreads_or(lost)) {"):]
+        end = end[:end.index("tcgen05.dealloc")]
+        for wait in copies + ("umma_commit(bar", "mbar_wait(bar"):
+            assert wait in end, (name, wait)
+    assert re.search(r"if \(lost\) \{[^}]*mbar_wait\(bar_image, 0\), mbar_wait\(bar_mma, 0\);", source("tq_tree.cu"))

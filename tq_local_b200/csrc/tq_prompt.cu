@@ -41,7 +41,7 @@ constexpr int kPolyOf8 = 2;
 constexpr int kSlotBytes = kUmmaTermBytes;       // 128 rows x 128 16-bit values
 constexpr int kSlots = 5;
 // two query tiles, the ring, barriers and the TMEM address
-constexpr int kBarsAt = (2 + kSlots) * kSlotBytes, kBars = 2 + 4 + 4 + 2 + 2 * kSlots + 3;
+constexpr int kBarsAt = (2 + kSlots) * kSlotBytes, kBars = 2 + 4 + 4 + 2 + 2 * kSlots + 3 + 2;
 constexpr int kSmem = kBarsAt + 8 * kBars + 16;
 
 struct PromptArgs {
@@ -109,12 +109,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const uint32_t base = smem_u32(smem_raw), ring = base + 2 * kSlotBytes, bars = base + kBarsAt;
     uint32_t *const s_tmem = reinterpret_cast<uint32_t *>(smem_raw + kBarsAt + 8 * kBars);
+    int *const s_asked = reinterpret_cast<int *>(s_tmem + 1);  // copies that were requested: of keys and values, and of which tiles' queries
     if (base & 1023u) {
         if (threadIdx.x == 0) atomicExch(&g_prompt_status, 2);
         return;
     }
-    // q: queries are there; s[tile][unit & 1]: logits are there; p[tile][unit & 1]: weights are there; o[tile]: O += P V is done; full, empty: slots
-    const uint32_t bar_q = bars, bar_s = bars + 16, bar_p = bars + 48, bar_o = bars + 80, bar_full = bars + 96, bar_empty = bar_full + 8 * kSlots, bar_ask = bar_empty + 8 * kSlots, bar_clean = bar_ask + 8;
+    // q: queries are there; s[tile][unit & 1]: logits are there; p[tile][unit & 1]: weights are there; o[tile]: O += P V is done; full, empty: slots;
+    // done[tile]: see the end
+    const uint32_t bar_q = bars, bar_s = bars + 16, bar_p = bars + 48, bar_o = bars + 80, bar_full = bars + 96, bar_empty = bar_full + 8 * kSlots, bar_ask = bar_empty + 8 * kSlots, bar_clean = bar_ask + 8, bar_done = bar_clean + 16;
     const int tid = threadIdx.x, warp = tid >> 5;
     if (warp == kSoftmax / 32 + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)), "r"(512));
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kSoftmax / 32 && elect_one()) {
         mbar_init(bar_q, 1), mbar_init(bar_q + 8, 1), mbar_init(bar_ask, 1), mbar_init(bar_clean, 1), mbar_init(bar_clean + 8, 1);
         for (int i = 0; i < 4; ++i) mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 4);
-        for (int w = 0; w < 2; ++w) mbar_init(bar_o + 8 * w, 1);
+        for (int w = 0; w < 2; ++w) mbar_init(bar_o + 8 * w, 1), mbar_init(bar_done + 8 * w, 1);
         for (int s = 0; s < kSlots; ++s) mbar_init(bar_full + 8 * s, 1), mbar_init(bar_empty + 8 * s, 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -163,10 +165,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == kSoftmax / 32) {
             // ---------------- copies
             if (elect_one()) {
-                for (int i = kSlots; i < 2 * nb; ++i) {
+                int i = kSlots;
+                for (; i < 2 * nb; ++i) {
                     wait(bar_empty + 8 * (i % kSlots), (i / kSlots & 1) ^ 1);
+                    if (lost) break;
                     load_slot(i);
                 }
+                s_asked[0] = min(2 * nb, i), s_asked[1] = (nu0 > 0) | (nu1 > 0) << 1;
             }
         } else if (warp < kSoftmax / 32 + 3) {
             // ---------------- products of tile w.  A wait costs a thread some 200 cycles even when there is nothing to wait for; a warp a tile keeps
@@ -396,9 +401,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             copy_rows(live ? dst : 0);
         }
     }
-    if (lost) atomicExch(&g_prompt_status, 1);
     umma_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(lost)) {
+        // A thread whose wait ran out waits for nothing more.  What was set going ends before the CTA does all the same: a copy that landed later would land in
+        // another's shared memory.
+        if (lost) atomicExch(&g_prompt_status, 1);
+        if (warp == kSoftmax / 32 && elect_one()) {
+            for (int i = max(s_asked[0] - kSlots, 0); i < s_asked[0]; ++i) mbar_wait(bar_full + 8 * (i % kSlots), i / kSlots & 1);
+            for (int w = 0; w < 2; ++w)
+                if (s_asked[1] >> w & 1) mbar_wait(bar_q + 8 * w, 0);
+        } else if (warp > kSoftmax / 32 && warp < kSoftmax / 32 + 3 && elect_one()) {
+            const uint32_t bar = bar_done + 8 * (warp - kSoftmax / 32 - 1);
+            umma_commit(bar);
+            mbar_wait(bar, 0);
+        }
+        __syncthreads();
+    }
     if (warp == kSoftmax / 32 + 1) {
         umma_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));

@@ -188,7 +188,10 @@ struct RowTile {
         umma_fence_after();
     }
     __device__ __forceinline__ void finish(int *error_flag) {
-        if (lost) atomicExch(error_flag, 8);
+        if (lost) {  // the matrix may still be on its way, the product under way
+            mbar_wait(bar_image, 0), mbar_wait(bar_mma, 0);
+            atomicExch(error_flag, 8);
+        }
         umma_fence_before();
         __syncthreads();
         if (threadIdx.x < 32) {
@@ -290,7 +293,7 @@ __device__ __forceinline__ uint32_t seen_word(const Entry &e, uint64_t mask, int
 template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 1) tq_tree_kernel(const __grid_constant__ TreeArgs a) {
     using L = Layout<KB, VB, QJL>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 1 + 1 + 1 + 2 + 2 * kRingSlots];
+    __shared__ uint64_t s_bars[2 + 2 + 2 + 2 + 1 + 1 + 1 + 2 + 2 * kRingSlots + 1];
     __shared__ uint32_t s_tmem;
     // What two warps that share rows tell each other, [block parity][half][row].  Two copies: one warp may be at the next block's logits while the other has
     // not yet read the maximum of this one (the products for them do not wait for this block's weights), but no further ahead than that.
@@ -298,9 +301,9 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = smem_u32(s_bars);
     // kfull, vfull: operands are there; kfree, vfree: the products that read keys and signs, or values, are done; s: logits are there; p: weights are there; o: O += P V is
-    // done; q: queries are there; raw, read: a slot of the ring is filled, has been read
+    // done; q: queries are there; raw, read: a slot of the ring is filled, has been read; done: see the end
     const uint32_t bar_kfull = bars, bar_kfree = bars + 16, bar_s = bars + 32, bar_p = bars + 48, bar_o = bars + 64, bar_q = bars + 72, bar_vfull = bars + 80, bar_vfree = bars + 88,
-                   bar_raw = bars + 104, bar_read = bar_raw + 8 * kRingSlots;
+                   bar_raw = bars + 104, bar_read = bar_raw + 8 * kRingSlots, bar_done = bar_read + 8 * kRingSlots;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int kProducts = kSoftmaxWarps + kOperandWarps;
     const int row_warps = (a.rows + 31) >> 5;  // quarters of the tile that have rows (the others' rows of S and O are what they are)
@@ -313,7 +316,7 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             mbar_init(bar_kfull + 8 * i, kOperandWarps / 2), mbar_init(bar_kfree + 8 * i, 1), mbar_init(bar_vfree + 8 * i, 1);
             mbar_init(bar_s + 8 * i, 1), mbar_init(bar_p + 8 * i, 2 * row_warps);
         }
-        mbar_init(bar_o, 1), mbar_init(bar_q, 2 * row_warps), mbar_init(bar_vfull, kOperandWarps / 2);
+        mbar_init(bar_done, 1), mbar_init(bar_o, 1), mbar_init(bar_q, 2 * row_warps), mbar_init(bar_vfull, kOperandWarps / 2);
         for (int i = 0; i < kRingSlots; ++i) mbar_init(bar_raw + 8 * i, 1), mbar_init(bar_read + 8 * i, kOperandWarps / 2);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -387,6 +390,7 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
     auto wait = [&](uint32_t bar, uint32_t parity) {
         if (!lost && !mbar_wait(bar, parity)) lost = true;
     };
+    uint32_t asked = 0;  // packed blocks that were requested
 
     if (warp >= kProducts) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
@@ -427,14 +431,15 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
         } else if (warp == kProducts + 1) {
             // ---------------- packed blocks: bulk copies of whole eights of tokens, kRingSlots blocks ahead
             if (elect_one()) {
-                uint32_t n = 0;
-                while (flat < flat_end) {
+                uint32_t &n = asked;
+                while (flat < flat_end && !lost) {
                     const Segment g = next_segment();
                     const int64_t row = g.b * a.cache_sb + g.h * a.cache_sh;
                     const int tree = up8(g.e.end), tree_end = tree + up8((a.tree_start & 7) + a.nodes);  // places of the second run of tokens
                     for (int k = g.k; k < g.k_end; ++k, ++n) {
                         const int slot = n % kRingSlots, at = k * kBlock;
                         if (n >= kRingSlots) wait(bar_read + 8 * slot, (n / kRingSlots & 1) ^ 1);
+                        if (lost) break;
                         const uint32_t bar = bar_raw + 8 * slot, dst = base + L::kRing + slot * L::kSlot;
                         const int n0 = max(min(kBlock, tree - at), 0), n1 = max(min(kBlock, tree_end - at) - n0, 0);
 #ifdef TQ_DEBUG_BOUNDS
@@ -693,9 +698,19 @@ template <int KB, int VB, bool QJL> __global__ void __launch_bounds__(kThreads, 
             pair_sync();  // (the sums have been read)
         }
     }
-    if (lost) atomicExch(a.error_flag, 8);
     umma_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(lost)) {
+        // A thread whose wait ran out waits for nothing more.  What was set going ends before the CTA does all the same: a copy that landed later would land in
+        // another's shared memory.
+        if (lost) atomicExch(a.error_flag, 8);
+        if (warp == kProducts && elect_one()) {
+            umma_commit(bar_done);
+            mbar_wait(bar_done, 0);
+        } else if (warp == kProducts + 1 && elect_one()) {
+            for (uint32_t i = asked > kRingSlots ? asked - kRingSlots : 0; i < asked; ++i) mbar_wait(bar_raw + 8 * (i % kRingSlots), i / kRingSlots & 1);
+        }
+        __syncthreads();
+    }
     if (warp == kProducts) {
         umma_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
