@@ -14,7 +14,7 @@
 // are outside the sequence.  S = Q K^T with both operands in shared memory; the weights go back to TMEM over S as 16-bit pairs and are the A
 // operand of O += P V.  TMEM: S of the two tiles, O of the two tiles, 128 columns each.
 //
-// What bounds it: 32768 tokens, 32 / 8 heads, bf16, take 7.3 ms on a card at rest (1200 TFLOP/s) and 8.4 ms back to back, where the card's
+// What bounds it: 32768 tokens, 32 / 8 heads, bf16, take 7.4 ms on a card at rest (1190 TFLOP/s) and 8.4 ms back to back, where the card's
 // power limit lowers its clock (1050; the library's matrix product falls from 1657 to 1376).  Between steps the tensor core waits for exponentials
 // (16 a clock and SM against 8192 operations: as long as the products) and for the hand-over of logits and weights.
 #include <cuda.h>

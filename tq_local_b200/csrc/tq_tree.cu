@@ -25,6 +25,7 @@
 // all four left out 109 remain, which is the hand-over from role to role.  Shared memory is three quarters busy (operands written once and read once by the
 // products, which read all of B again for every 128 rows).  Variants measured on the way: operands by eight warps straight from
 // global memory, two stages of everything, 197 us; by sixteen, one block at a time, 247; two stages of values and two of the ring, 227.
+// 896 threads are launched with 72 registers each, at which 184 to 232 bytes a thread are spilled.
 #include <math.h>
 
 #include <type_traits>

@@ -426,7 +426,7 @@ class PackedStore:
         history ``[seq_start[b], lengths[b])`` (``lengths``: int32 [B] on the device; default: all of ``[0, tree_start)``) and,
         of the drafted tokens, those whose bits are set in ``tree_mask`` (int64 [B, T], or [T] for all rows; bit j of
         word i: node i sees node j; T at most 64).  Without a mask they are a chain: node i sees nodes 0 .. i, any T.  With
-        T = 1 and no mask this is single-token decoding of rows of different lengths."""
+        T = 1 and no mask this is single-token decoding of rows of different lengths (rows of one length: ``decode_attn`` is faster)."""
         if q.dim() != 4 or q.shape[0] != self.batch or q.shape[-1] != 128 or q.shape[1] % self.kv_heads:
             raise ValueError(f"expected queries [B={self.batch}, Hq, T, 128] with Hq a multiple of {self.kv_heads}, got {tuple(q.shape)}")
         if q.device != self.codec.device:
