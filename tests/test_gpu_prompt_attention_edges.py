@@ -45,6 +45,7 @@ def test_the_status_waits_for_every_stream():
     from tq_local_b200.runtime.prompt_attention import prompt_attention, raise_on_status
 
     q = torch.zeros(1, 2, 8, 128, device="cuda", dtype=BF16)
+    prompt_attention(q, q, q)  # (loads the kernel)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):

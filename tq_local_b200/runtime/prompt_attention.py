@@ -108,7 +108,7 @@ def prompt_attention_packed(query: torch.Tensor, key: torch.Tensor, value: torch
 
 def raise_on_status(device: torch.device, where: str) -> None:
     """Raise :class:`TQError` when a prompt kernel of this device has given up waiting (synchronises with the device).  What is reported is
-    cleared: later calls are judged by themselves."""
+    cleared: it says nothing of later calls."""
     v = C.c_int32()
     with torch.cuda.device(device):
         ffi.check(ffi.lib().tq_prompt_status(C.byref(v)), "tq_prompt_status")
